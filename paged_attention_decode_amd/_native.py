@@ -179,6 +179,76 @@ SIGNATURES = {
 }
 
 
+class PadCacheCall(ctypes.Structure):
+    """``pad_cache_call`` of include/pa_cache.h."""
+
+    _fields_ = [
+        ("call", PadCall),
+        ("k_scales", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("ks_stride", ctypes.c_int64 * 3),
+        ("vs_stride", ctypes.c_int64 * 3),
+        ("weights", ctypes.c_void_p),
+        ("w_stride", ctypes.c_int64 * 3),
+        ("logits", ctypes.c_void_p),
+        ("logits_bytes", ctypes.c_size_t),
+    ]
+
+
+class PadKvCache(ctypes.Structure):
+    """``pad_kv_cache`` of include/pa_cache.h."""
+
+    _fields_ = [
+        *[(name, ctypes.c_void_p) for name in ("k", "v", "k_scales", "v_scales", "weights", "positions")],
+        *[(name, ctypes.c_int64 * 3)
+          for name in ("k_stride", "v_stride", "ks_stride", "vs_stride", "w_stride", "p_stride")],
+        ("num_pages", ctypes.c_int64),
+        *[(name, ctypes.c_int32) for name in ("page_size", "num_kv_heads", "head_dim", "kv_format")],
+        ("k_scale", ctypes.c_float),
+        ("v_scale", ctypes.c_float),
+    ]
+
+
+class PadKvRows(ctypes.Structure):
+    """``pad_kv_rows`` of include/pa_cache.h."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_stride", ctypes.c_int64 * 2),
+        ("v_stride", ctypes.c_int64 * 2),
+        ("slots", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("slots64", ctypes.c_int32),
+        ("bf16", ctypes.c_int32),
+    ]
+
+
+class PadKvEvictCall(ctypes.Structure):
+    """``pad_kv_evict_call`` of include/pa_cache.h."""
+
+    _fields_ = [
+        *[(name, ctypes.c_void_p) for name in ("block_table", "seq_lens", "keeps", "new_lens", "workspace")],
+        ("workspace_bytes", ctypes.c_size_t),
+        ("bt_stride", ctypes.c_int64 * 2),
+        ("sl_stride", ctypes.c_int64),
+        *[(name, ctypes.c_int32) for name in ("batch", "max_pages", "keep", "recent")],
+    ]
+
+
+# include/pa_cache.h
+CACHE_SIGNATURES = {
+    "pad_cache_logits_bytes": ([ctypes.POINTER(PadDims), ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    "pad_cache_decode": ([ctypes.POINTER(PadCacheCall), ctypes.POINTER(PadDims), _VP], ctypes.c_int),
+    "pad_kv_append": ([ctypes.POINTER(PadKvCache), ctypes.POINTER(PadKvRows), _VP, _VP, _VP], ctypes.c_int),
+    "pad_kv_read": ([ctypes.POINTER(PadKvCache), ctypes.POINTER(PadKvRows), _VP], ctypes.c_int),
+    "pad_kv_evict_workspace_bytes": (
+        [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_size_t)],
+        ctypes.c_int),
+    "pad_kv_evict": ([ctypes.POINTER(PadKvCache), ctypes.POINTER(PadKvEvictCall), _VP], ctypes.c_int),
+}
+
+
 def capi():
     """ctypes handle to libpa_decode.so with typed entry points (loaded once)."""
     global _capi
@@ -186,7 +256,7 @@ def capi():
         if not os.path.exists(CAPI_PATH):
             raise ImportError(f"paged_attention_decode_amd: {CAPI_PATH} is missing; {_BUILD_HINT}")
         lib = ctypes.CDLL(CAPI_PATH)
-        for name, (argtypes, restype) in SIGNATURES.items():
+        for name, (argtypes, restype) in {**SIGNATURES, **CACHE_SIGNATURES}.items():
             fn = getattr(lib, name)
             fn.argtypes = argtypes
             fn.restype = restype

@@ -4,8 +4,8 @@ Four shared libraries, all written next to this file (and one test program,
 below):
 
 * ``libpa_decode.so`` - the C-ABI library (``include/pa_decode.h``): gfx950
-  kernels plus ``extern "C"`` entry points, compiled by ``hipcc`` from
-  ``csrc/pa_decode.hip`` and ``csrc/pa_range.hip``.
+  kernels plus ``extern "C"`` entry points (``include/pa_decode.h``,
+  ``include/pa_cache.h``), compiled by ``hipcc`` from ``CAPI_SOURCES``.
 * ``_pa_decode_ext<EXT_SUFFIX>`` - the thin PyTorch binding
   (``csrc/pa_torch.cpp``), host-only C++ compiled by ``g++`` against
   PyTorch's headers and linked to ``libpa_decode.so`` through an
@@ -41,7 +41,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(REPO_DIR, "include")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 ARCH = "gfx950"
-CAPI_SOURCES = ("pa_decode", "pa_range")  # csrc/*.hip of libpa_decode.so
+CAPI_SOURCES = ("pa_decode", "pa_range", "pa_cache", "pa_mx4", "pa_weights", "pa_weights_fp8")  # csrc/*.hip of libpa_decode.so
 
 CAPI_LIB = os.path.join(PKG_DIR, "libpa_decode.so")
 PROBE_LIB = os.path.join(PKG_DIR, "libpa_probe.so")

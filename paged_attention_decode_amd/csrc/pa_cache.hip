@@ -1,0 +1,695 @@
+// pa_cache.hip - gfx950 kernels that write, read and thin out a paged K/V cache:
+// append, read, the accumulation of attention weights, and eviction
+// (include/pa_cache.h).
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "pa_cache.h"
+#include "pa_device.h"
+#include "pa_ext.h"
+
+namespace pad {
+
+typedef float f2_t __attribute__((ext_vector_type(2)));
+
+// ---------------------------------------------------------------------------
+// Append and read.  A thread has eight elements of a row (16 bytes of 16-bit
+// values); the four lanes of an MX4 block find its largest value together.  Bound
+// by memory: the rows are read (or written) once, the cache's the other way.
+// ---------------------------------------------------------------------------
+constexpr int kRows16 = 0, kRowsE4M3 = 1, kRowsE5M2 = 2, kRowsMx4 = 3;  // kinds of cache rows
+
+struct RowArgs {
+  pad_kv_cache c;
+  pad_kv_rows r;
+  const float* token_weights;
+  const int32_t* token_positions;
+  int64_t work;  // tokens * kv heads * (head_dim / 8)
+  int row8;      // head_dim / 8
+  int ps_shift;
+};
+
+__device__ __forceinline__ int64_t slot_of(const RowArgs& a, int64_t token) {
+  return a.r.slots64 ? static_cast<const int64_t*>(a.r.slots)[token] : static_cast<const int32_t*>(a.r.slots)[token];
+}
+
+// Page and place of a slot; false for one outside the cache.
+__device__ __forceinline__ bool place_of(const RowArgs& a, int64_t s, int64_t& page, int64_t& at) {
+  if (s < 0) return false;
+  if (a.ps_shift >= 0) {
+    page = s >> a.ps_shift;
+  } else if (s < (1ll << 32)) {
+    page = (uint32_t)s / (uint32_t)a.c.page_size;
+  } else {
+    page = s / a.c.page_size;
+  }
+  at = s - page * a.c.page_size;
+  return page < a.c.num_pages;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void unpack8(u4_t w, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BF16) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const h2_t h = __builtin_bit_cast(h2_t, (uint32_t)w[i]);
+      x[2 * i] = (float)h.x;
+      x[2 * i + 1] = (float)h.y;
+    }
+  }
+}
+
+template <bool BF16>
+__device__ __forceinline__ u4_t pack8(const float (&x)[8]) {
+  u4_t w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BF16) {
+      typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+      w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2_t{x[2 * i], x[2 * i + 1]}, b2_t));
+    } else {
+      w[i] = __builtin_bit_cast(uint32_t, h2_t{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
+    }
+  }
+  return w;
+}
+
+// Four values / scale as fp8 codes, held to the largest finite value (a
+// comparison with NaN is false, so NaN stays).
+template <int KIND>
+__device__ __forceinline__ uint32_t fp8x4(const float* x, float scale) {
+  constexpr float kMax = KIND == kRowsE4M3 ? 448.f : 57344.f;
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float v = x[i] / scale;
+    y[i] = v > kMax ? kMax : (v < -kMax ? -kMax : v);
+  }
+  int w = 0;
+  if constexpr (KIND == kRowsE4M3) {
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], w, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+  } else {
+    w = __builtin_amdgcn_cvt_pk_bf8_f32(y[0], y[1], w, false);
+    w = __builtin_amdgcn_cvt_pk_bf8_f32(y[2], y[3], w, true);
+  }
+  return (uint32_t)w;
+}
+
+template <int KIND, bool BF16>
+__global__ __launch_bounds__(256) void pad_append_kernel(const RowArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const bool is_v = blockIdx.y != 0;
+  // Rows have whole groups of four threads, so a block's lanes live or leave
+  // together.
+  if (i >= a.work) return;
+  const int64_t row = i / a.row8;
+  const int e8 = (int)(i - row * a.row8);
+  const int64_t token = row / a.c.num_kv_heads;
+  const int h = (int)(row - token * a.c.num_kv_heads);
+  const _Float16* src = static_cast<const _Float16*>(is_v ? a.r.v : a.r.k) +
+                        token * (is_v ? a.r.v_stride[0] : a.r.k_stride[0]) +
+                        (int64_t)h * (is_v ? a.r.v_stride[1] : a.r.k_stride[1]) + e8 * 8;
+  const u4_t w = __builtin_nontemporal_load(reinterpret_cast<const u4_t*>(src));
+  int64_t page, at;
+  if (!place_of(a, slot_of(a, token), page, at)) return;
+  const int64_t* st = is_v ? a.c.v_stride : a.c.k_stride;
+  const int64_t off = page * st[0] + at * st[1] + (int64_t)h * st[2];
+  char* base = static_cast<char*>(is_v ? a.c.v : a.c.k);
+  if constexpr (KIND == kRows16) {
+    *reinterpret_cast<u4_t*>(base + (off + e8 * 8) * 2) = w;
+  } else {
+    float x[8];
+    unpack8<BF16>(w, x);
+    if constexpr (KIND == kRowsMx4) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+      top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
+      const int e = (int)(top >> 23);  // biased; 255: NaN or infinity
+      const uint32_t s = e == 255 ? 255u : (uint32_t)max(e - 2, 0);
+      // v_cvt_scalef32_pk_fp4_f32 divides by the scale, rounds to nearest even
+      // and saturates (exponent byte 0 stands for 2^-127).
+      const float scale = __uint_as_float(s << 23);
+      uint32_t codes = 0;
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], scale, 0);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], scale, 1);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], scale, 2);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], scale, 3);
+      *reinterpret_cast<uint32_t*>(base + off + e8 * 4) = e == 255 ? 0u : codes;
+      if ((e8 & 3) == 0) {
+        const int64_t* ss = is_v ? a.c.vs_stride : a.c.ks_stride;
+        (is_v ? a.c.v_scales : a.c.k_scales)[page * ss[0] + at * ss[1] + (int64_t)h * ss[2] + (e8 >> 2)] = (uint8_t)s;
+      }
+    } else {
+      const float scale = is_v ? a.c.v_scale : a.c.k_scale;
+      *reinterpret_cast<u2_t*>(base + off + e8 * 8) = u2_t{fp8x4<KIND>(x, scale), fp8x4<KIND>(x + 4, scale)};
+    }
+  }
+  if (e8 == 0) {
+    if (!is_v && a.c.weights)
+      a.c.weights[page * a.c.w_stride[0] + at * a.c.w_stride[1] + (int64_t)h * a.c.w_stride[2]] =
+          a.token_weights ? a.token_weights[row] : 0.f;
+    if (is_v && a.c.positions)
+      a.c.positions[page * a.c.p_stride[0] + at * a.c.p_stride[1] + (int64_t)h * a.c.p_stride[2]] =
+          a.token_positions[token];
+  }
+}
+
+template <int KIND, bool BF16>
+__global__ __launch_bounds__(256) void pad_read_kernel(const RowArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const bool is_v = blockIdx.y != 0;
+  if (i >= a.work) return;
+  const int64_t row = i / a.row8;
+  const int e8 = (int)(i - row * a.row8);
+  const int64_t token = row / a.c.num_kv_heads;
+  const int h = (int)(row - token * a.c.num_kv_heads);
+  _Float16* dst = static_cast<_Float16*>(is_v ? a.r.v : a.r.k) + token * (is_v ? a.r.v_stride[0] : a.r.k_stride[0]) +
+                  (int64_t)h * (is_v ? a.r.v_stride[1] : a.r.k_stride[1]) + e8 * 8;
+  int64_t page, at;
+  u4_t out = (u4_t)0u;
+  if (place_of(a, slot_of(a, token), page, at)) {
+    const int64_t* st = is_v ? a.c.v_stride : a.c.k_stride;
+    const int64_t off = page * st[0] + at * st[1] + (int64_t)h * st[2];
+    const char* base = static_cast<const char*>(is_v ? a.c.v : a.c.k);
+    if constexpr (KIND == kRows16) {
+      out = *reinterpret_cast<const u4_t*>(base + (off + e8 * 8) * 2);
+    } else if constexpr (KIND == kRowsMx4) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(base + off + e8 * 4);
+      const int64_t* ss = is_v ? a.c.vs_stride : a.c.ks_stride;
+      const uint32_t s = (is_v ? a.c.v_scales
+                               : a.c.k_scales)[page * ss[0] + at * ss[1] + (int64_t)h * ss[2] + (e8 >> 2)];
+      const float scale = __uint_as_float(s << 23);
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f2_t p = j == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0)
+                       : j == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1)
+                       : j == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 2)
+                                : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 3);
+        x[2 * j] = p.x;
+        x[2 * j + 1] = p.y;
+      }
+      out = pack8<BF16>(x);
+    } else {
+      const u2_t w = *reinterpret_cast<const u2_t*>(base + off + e8 * 8);
+      const float scale = is_v ? a.c.v_scale : a.c.k_scale;
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        f2_t lo, hi;
+        if constexpr (KIND == kRowsE4M3) {
+          lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j], false);
+          hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j], true);
+        } else {
+          lo = __builtin_amdgcn_cvt_pk_f32_bf8((int)w[j], false);
+          hi = __builtin_amdgcn_cvt_pk_f32_bf8((int)w[j], true);
+        }
+        x[4 * j] = lo.x * scale;
+        x[4 * j + 1] = lo.y * scale;
+        x[4 * j + 2] = hi.x * scale;
+        x[4 * j + 3] = hi.y * scale;
+      }
+      out = pack8<BF16>(x);
+    }
+  }
+  __builtin_nontemporal_store(out, reinterpret_cast<u4_t*>(dst));
+}
+
+// ---------------------------------------------------------------------------
+// weights[slot] += sum over the group's rows of 2^(score - lse): the second
+// half of a kKvWeights decode.  A workgroup walks tokens of one (sequence, kv
+// head) unit; each weight is updated by one thread, so the sums have one order.
+// ---------------------------------------------------------------------------
+struct AccumulateArgs {
+  const float* logits;
+  const float* lse;
+  const int32_t* bt;
+  const int32_t* sl;
+  float* weights;
+  int64_t slog, sbb, sbp, ssl, swp, sws, swh, num_pages;
+  int gqa, hkv, ps, ps_shift, max_pages;
+};
+
+__global__ __launch_bounds__(256) void pad_accumulate_kernel(const AccumulateArgs a) {
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int64_t cap = (int64_t)a.max_pages * a.ps;
+  const int64_t L = min((int64_t)max(a.sl[(int64_t)b * a.ssl], 0), cap);
+  const int64_t row0 = ((int64_t)b * a.hkv + h) * a.gqa;
+  const float* x = a.logits + row0 * a.slog;
+  const float* lse = a.lse + row0;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < L; t += (int64_t)gridDim.x * 256) {
+    const int64_t page = a.ps_shift >= 0 ? t >> a.ps_shift : (int64_t)((uint32_t)t / (uint32_t)a.ps);
+    const int64_t id = clamp_page(a.bt[b * a.sbb + page * a.sbp], a.num_pages);
+    float* w = a.weights + id * a.swp + (t - page * a.ps) * a.sws + (int64_t)h * a.swh;
+    float sum = 0.f;
+    for (int r = 0; r < a.gqa; ++r) sum += exp2_fast(x[(int64_t)r * a.slog + t] - lse[r]);
+    *w += sum;
+  }
+}
+
+hipError_t launch_accumulate(const Phase1Args& p, float* weights, const int64_t* w_stride, hipStream_t st) {
+  AccumulateArgs a = {};
+  a.logits = p.logits;
+  a.lse = p.lse;
+  a.bt = p.bt;
+  a.sl = p.sl;
+  a.weights = weights;
+  a.slog = p.slog;
+  a.sbb = p.sbb;
+  a.sbp = p.sbp;
+  a.ssl = p.ssl;
+  a.swp = w_stride[0];
+  a.sws = w_stride[1];
+  a.swh = w_stride[2];
+  a.num_pages = p.num_pages;
+  a.gqa = p.gqa;
+  a.hkv = p.hkv;
+  a.ps = p.ps;
+  a.ps_shift = p.ps_shift;
+  a.max_pages = p.max_pages;
+  const int64_t units = (int64_t)p.batch * p.hkv;
+  const int64_t chunks = ((int64_t)p.max_pages * p.ps + 255) / 256;
+  const int64_t most = 4096 / units > 1 ? 4096 / units : 1;
+  hipLaunchKernelGGL(pad_accumulate_kernel, dim3((unsigned)(chunks < most ? chunks : most), p.hkv, p.batch), dim3(256),
+                     0, st, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Eviction.  Per (sequence, kv head): the keep-th largest key by radix selection
+// (three digits of 11, 11 and 10 bits of an order-preserving integer of the
+// weight), ties by slot order, then the list of moves: the i-th kept slot at or
+// above the new length goes to the i-th evicted slot below it.  Sources lie at or
+// above the new length and targets below it, so no move can overwrite what
+// another reads, and moves run in any order.
+// ---------------------------------------------------------------------------
+struct EvictArgs {
+  pad_kv_cache c;
+  pad_kv_evict_call e;
+  int2* moves;     // [units][most] (source slot, target slot)
+  int* num_moves;  // [units]
+  int64_t most;
+  int ps_shift;
+  int row_units;   // vector units of a K (or V) row
+  int elem_bytes;  // bytes per element of the rows' strides
+  int scale_bytes; // MX4 scale bytes of a row, else 0
+};
+
+constexpr int kEvictThreads = 1024;
+constexpr int kEvictWaves = kEvictThreads / 64;
+constexpr uint32_t kKeyNewest = 0xffffffffu;
+constexpr uint32_t kKeyNan = 0xfffffffeu;
+
+// Order-preserving integer of a weight (-0 counts as 0); 0 is below all.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  if (w != w) return kKeyNan;
+  const uint32_t u = __float_as_uint(w + 0.f);
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ int evict_page(const EvictArgs& a, int slot) {
+  return a.ps_shift >= 0 ? slot >> a.ps_shift : (int)((uint32_t)slot / (uint32_t)a.c.page_size);
+}
+
+// Offset helper: where a slot of sequence b lies.
+struct Place {
+  int64_t page, at;
+};
+__device__ __forceinline__ Place evict_place(const EvictArgs& a, int b, int slot) {
+  const int page = evict_page(a, slot);
+  Place p;
+  p.page = clamp_page(a.e.block_table[(int64_t)b * a.e.bt_stride[0] + (int64_t)page * a.e.bt_stride[1]], a.c.num_pages);
+  p.at = slot - (int64_t)page * a.c.page_size;
+  return p;
+}
+
+// Exclusive prefix of one count per wave, and their total (every thread calls it).
+__device__ __forceinline__ int wave_base(int count, int wave, int* sm, int& total) {
+  if ((threadIdx.x & 63) == 0) sm[wave] = count;
+  __syncthreads();
+  int base = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kEvictWaves; ++w) {
+    const int c = sm[w];
+    base += w < wave ? c : 0;
+    all += c;
+  }
+  total = all;
+  __syncthreads();
+  return base;
+}
+
+__global__ __launch_bounds__(kEvictThreads) void pad_evict_select_kernel(const EvictArgs a) {
+  const int h = blockIdx.x, b = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t unit = (int64_t)b * a.c.num_kv_heads + h;
+  const int64_t cap = (int64_t)a.e.max_pages * a.c.page_size;
+  const int L = (int)min((int64_t)max(a.e.seq_lens[(int64_t)b * a.e.sl_stride], 0), cap);
+  const int n = min(max(a.e.keeps ? a.e.keeps[b] : a.e.keep, 0), L);
+  if (tid == 0 && h == 0) a.e.new_lens[b] = n;
+  if (n == L || n == 0) {
+    if (tid == 0) a.num_moves[unit] = 0;
+    return;
+  }
+  __shared__ int hist[2048];
+  __shared__ int sm[kEvictWaves];
+  __shared__ int s_bin, s_above;
+
+  // A wave has consecutive slots, 64 at a time.
+  const int steps = (L + kEvictThreads - 1) / kEvictThreads;
+  const int first = wave * steps * 64 + lane;
+  auto weight_at = [&](int slot) {
+    const Place p = evict_place(a, b, slot);
+    return a.c.weights[p.page * a.c.w_stride[0] + p.at * a.c.w_stride[1] + (int64_t)h * a.c.w_stride[2]];
+  };
+  auto position_at = [&](int slot) {
+    const Place p = evict_place(a, b, slot);
+    return a.c.positions[p.page * a.c.p_stride[0] + p.at * a.c.p_stride[1] + (int64_t)h * a.c.p_stride[2]];
+  };
+  int newest = INT32_MIN;
+  for (int i = 0; i < steps; ++i) {
+    const int slot = first + i * 64;
+    if (slot < L) newest = max(newest, position_at(slot));
+  }
+  newest = wave_max_i32(newest);
+  if (lane == 0) sm[wave] = newest;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kEvictWaves; ++w) newest = max(newest, sm[w]);
+  __syncthreads();
+  const int64_t border = (int64_t)newest - a.e.recent;
+  auto key_at = [&](int slot) -> uint32_t {
+    if (slot >= L) return 0u;
+    if ((int64_t)position_at(slot) > border) return kKeyNewest;
+    return weight_key(weight_at(slot));
+  };
+
+  // The n-th largest key.
+  uint32_t prefix = 0, mask = 0;
+  int left = n;  // of the keys with this prefix, how many from the top
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t bins = pass == 2 ? 1024u : 2048u;
+    for (int i = tid; i < 2048; i += kEvictThreads) hist[i] = 0;
+    __syncthreads();
+    for (int i = 0; i < steps; ++i) {
+      const uint32_t k = key_at(first + i * 64);
+      if (k != 0 && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+    }
+    __syncthreads();
+    // Thread t has bins 2047 - 2t and the one below: counts from the top.
+    const int hi = hist[2047 - 2 * tid], lo = hist[2046 - 2 * tid];
+    const int incl = wave_incl_scan_i32(hi + lo, lane);
+    int total;
+    const int base = wave_base(__builtin_amdgcn_readlane(incl, 63), wave, sm, total) + incl - hi - lo;
+    if (base < left && left <= base + hi) {
+      s_bin = 2047 - 2 * tid;
+      s_above = base;
+    } else if (base + hi < left && left <= base + hi + lo) {
+      s_bin = 2046 - 2 * tid;
+      s_above = base + hi;
+    }
+    __syncthreads();
+    prefix |= (uint32_t)s_bin << shift;
+    mask |= (bins - 1) << shift;
+    left -= s_above;
+    __syncthreads();
+  }
+  const uint32_t border_key = prefix;
+
+  // `left` of the keys equal to it are kept, the lowest slots first.
+  int ties = 0, total;
+  for (int i = 0; i < steps; ++i)
+    ties += (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key_at(first + i * 64) == border_key));
+  int tie = wave_base(ties, wave, sm, total);
+  const uint64_t below = (1ull << lane) - 1;
+  const int tie0 = tie;
+  int movers = 0, holes = 0;
+  for (int round = 0; round < 2; ++round) {
+    int mover = 0, hole = 0;
+    if (round == 1) {
+      mover = wave_base(movers, wave, sm, total);
+      hole = wave_base(holes, wave, sm, total);
+      tie = tie0;
+    }
+    for (int i = 0; i < steps; ++i) {
+      const int slot = first + i * 64;
+      const uint32_t k = key_at(slot);
+      const uint64_t eq = __builtin_amdgcn_ballot_w64(k == border_key);
+      const bool kept = k > border_key || (k == border_key && tie + (int)__builtin_popcountll(eq & below) < left);
+      tie += (int)__builtin_popcountll(eq);
+      const bool moves = kept && slot >= n, opens = !kept && slot < n;
+      const uint64_t mv = __builtin_amdgcn_ballot_w64(moves), op = __builtin_amdgcn_ballot_w64(opens);
+      if (round == 0) {
+        movers += (int)__builtin_popcountll(mv);
+        holes += (int)__builtin_popcountll(op);
+      } else {
+        int2* list = a.moves + unit * a.most;
+        const int m = mover + (int)__builtin_popcountll(mv & below), o = hole + (int)__builtin_popcountll(op & below);
+        if (moves && m < a.most) list[m].x = slot;
+        if (opens && o < a.most) list[o].y = slot;
+        mover += (int)__builtin_popcountll(mv);
+        hole += (int)__builtin_popcountll(op);
+      }
+    }
+  }
+  if (tid == 0) a.num_moves[unit] = (int)min((int64_t)total, a.most);
+}
+
+// Moves: TP = 2 * row_units threads per move (K's vector units, then V's).
+template <typename U>
+__global__ __launch_bounds__(256) void pad_evict_move_kernel(const EvictArgs a) {
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int64_t unit = (int64_t)b * a.c.num_kv_heads + h;
+  const int m = a.num_moves[unit];
+  const int tp = 2 * a.row_units;
+  const int per = 256 / tp;
+  const int mine = threadIdx.x / tp;
+  if (mine >= per) return;
+  const int task = threadIdx.x - mine * tp;
+  const bool is_v = task >= a.row_units;
+  const int c = is_v ? task - a.row_units : task;
+  const int64_t* st = is_v ? a.c.v_stride : a.c.k_stride;
+  const int64_t* ss = is_v ? a.c.vs_stride : a.c.ks_stride;
+  char* base = static_cast<char*>(is_v ? a.c.v : a.c.k) + (int64_t)h * st[2] * a.elem_bytes + c * sizeof(U);
+  const int2* list = a.moves + unit * a.most;
+  for (int i = blockIdx.x * per + mine; i < m; i += gridDim.x * per) {
+    const int2 mv = list[i];
+    const Place s = evict_place(a, b, mv.x), d = evict_place(a, b, mv.y);
+    *reinterpret_cast<U*>(base + (d.page * st[0] + d.at * st[1]) * a.elem_bytes) =
+        *reinterpret_cast<const U*>(base + (s.page * st[0] + s.at * st[1]) * a.elem_bytes);
+    if (c < a.scale_bytes) {
+      uint8_t* sb = (is_v ? a.c.v_scales : a.c.k_scales) + (int64_t)h * ss[2] + c;
+      sb[d.page * ss[0] + d.at * ss[1]] = sb[s.page * ss[0] + s.at * ss[1]];
+    }
+    if (c == 0) {
+      if (is_v) {
+        int32_t* p = a.c.positions + (int64_t)h * a.c.p_stride[2];
+        p[d.page * a.c.p_stride[0] + d.at * a.c.p_stride[1]] = p[s.page * a.c.p_stride[0] + s.at * a.c.p_stride[1]];
+      } else {
+        float* w = a.c.weights + (int64_t)h * a.c.w_stride[2];
+        w[d.page * a.c.w_stride[0] + d.at * a.c.w_stride[1]] = w[s.page * a.c.w_stride[0] + s.at * a.c.w_stride[1]];
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+static int shift_of(int ps) {
+  for (int sh = 0; sh < 31; ++sh)
+    if ((1 << sh) == ps) return sh;
+  return -1;
+}
+
+static int row_kind(int kv_format) {
+  switch (kv_format) {
+    case PAD_KV_FP16:
+    case PAD_KV_BF16: return kRows16;
+    case PAD_KV_FP8_E4M3FN: return kRowsE4M3;
+    case PAD_KV_FP8_E5M2: return kRowsE5M2;
+    case PAD_KV_MX4: return kRowsMx4;
+    default: return -1;
+  }
+}
+
+// Bytes of a row in the cache, and of a stride's element.
+static int row_bytes(const pad_kv_cache* c) {
+  const int kind = row_kind(c->kv_format);
+  return kind == kRows16 ? 2 * c->head_dim : kind == kRowsMx4 ? c->head_dim / 2 : c->head_dim;
+}
+static int stride_bytes(const pad_kv_cache* c) { return row_kind(c->kv_format) == kRows16 ? 2 : 1; }
+
+// Rows' alignment: the largest power of two (up to 16) that every row starts at.
+static int row_alignment(const pad_kv_cache* c) {
+  uint64_t x = (uint64_t)(uintptr_t)c->k | (uint64_t)(uintptr_t)c->v | 16u;
+  for (int i = 0; i < 3; ++i)
+    x |= (uint64_t)c->k_stride[i] * stride_bytes(c) | (uint64_t)c->v_stride[i] * stride_bytes(c);
+  return (int)(x & (~x + 1));
+}
+
+static int check_cache(const pad_kv_cache* c) {
+  if (!c || !c->k || !c->v) return PAD_ERR_NULL_POINTER;
+  const int kind = row_kind(c->kv_format);
+  if (kind < 0) return PAD_ERR_KV_FORMAT;
+  if (c->page_size <= 0 || c->num_kv_heads <= 0 || c->num_kv_heads > 65535 || c->num_pages <= 0 ||
+      c->num_pages > INT32_MAX)
+    return PAD_ERR_INVALID_SHAPE;
+  const int d = c->head_dim;
+  if (d != 64 && d != 128 && d != 256 && (kind != kRows16 || (d != 32 && d != 96))) return PAD_ERR_UNSUPPORTED_HEAD_DIM;
+  if (kind == kRowsMx4 && (!c->k_scales || !c->v_scales)) return PAD_ERR_NULL_POINTER;
+  if ((kind == kRowsE4M3 || kind == kRowsE5M2) &&
+      (!(c->k_scale > 0.f) || !(c->v_scale > 0.f) || c->k_scale > 1e30f || c->v_scale > 1e30f))
+    return PAD_ERR_KV_FORMAT;
+  const int need = kind == kRows16 ? 16 : 8;
+  return row_alignment(c) < need ? PAD_ERR_ALIGNMENT : PAD_OK;
+}
+
+static int check_rows(const pad_kv_cache* c, const pad_kv_rows* r) {
+  const int st = check_cache(c);
+  if (st != PAD_OK) return st;
+  if (!r) return PAD_ERR_NULL_POINTER;
+  if (r->tokens < 0) return PAD_ERR_INVALID_SHAPE;
+  if (r->tokens == 0) return PAD_OK;
+  if (!r->k || !r->v || !r->slots) return PAD_ERR_NULL_POINTER;
+  // A grid holds 2^31 - 1 workgroups of 256 threads.
+  if (r->tokens > ((int64_t)INT32_MAX * 256) / ((int64_t)c->num_kv_heads * (c->head_dim / 8)))
+    return PAD_ERR_INVALID_SHAPE;
+  if ((((uintptr_t)r->k | (uintptr_t)r->v) & 15u) != 0 ||
+      ((r->k_stride[0] | r->k_stride[1] | r->v_stride[0] | r->v_stride[1]) & 7) != 0)
+    return PAD_ERR_ALIGNMENT;
+  if (row_kind(c->kv_format) == kRows16 && (c->kv_format == PAD_KV_BF16) != (r->bf16 != 0)) return PAD_ERR_KV_FORMAT;
+  return PAD_OK;
+}
+
+template <template <int, bool> class K>
+static void launch_rows(const RowArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)((a.work + 255) / 256), 2);
+  const bool bf16 = a.r.bf16 != 0;
+  switch (row_kind(a.c.kv_format)) {
+    case kRows16: K<kRows16, false>::launch(a, grid, st); break;  // moved as bits
+    case kRowsE4M3: bf16 ? K<kRowsE4M3, true>::launch(a, grid, st) : K<kRowsE4M3, false>::launch(a, grid, st); break;
+    case kRowsE5M2: bf16 ? K<kRowsE5M2, true>::launch(a, grid, st) : K<kRowsE5M2, false>::launch(a, grid, st); break;
+    default: bf16 ? K<kRowsMx4, true>::launch(a, grid, st) : K<kRowsMx4, false>::launch(a, grid, st); break;
+  }
+}
+
+template <int KIND, bool BF16>
+struct Append {
+  static void launch(const RowArgs& a, dim3 grid, hipStream_t st) {
+    hipLaunchKernelGGL((pad_append_kernel<KIND, BF16>), grid, dim3(256), 0, st, a);
+  }
+};
+template <int KIND, bool BF16>
+struct Read {
+  static void launch(const RowArgs& a, dim3 grid, hipStream_t st) {
+    hipLaunchKernelGGL((pad_read_kernel<KIND, BF16>), grid, dim3(256), 0, st, a);
+  }
+};
+
+static RowArgs row_args(const pad_kv_cache* c, const pad_kv_rows* r) {
+  RowArgs a = {};
+  a.c = *c;
+  a.r = *r;
+  a.row8 = c->head_dim / 8;
+  a.work = r->tokens * c->num_kv_heads * a.row8;
+  a.ps_shift = shift_of(c->page_size);
+  return a;
+}
+
+// Slots of one sequence: the selection counts them, in steps of a workgroup, in
+// 32 bits.
+constexpr int64_t kMostSlots = INT32_MAX - 2 * kEvictThreads;
+
+// Workspace of an eviction: 256 bytes of slack, a count per unit, the move lists.  A unit of
+// capacity C moves at most C / 2 rows (sources at or above the new length,
+// targets below it).
+static int64_t most_moves(int64_t max_pages, int64_t page_size) { return max_pages * page_size / 2; }
+static size_t evict_counts_bytes(int64_t units) { return ((size_t)units * sizeof(int) + 255) & ~(size_t)255; }
+static size_t evict_bytes(int64_t units, int64_t max_pages, int64_t page_size) {
+  return 256 + evict_counts_bytes(units) + (size_t)(units * most_moves(max_pages, page_size)) * sizeof(int2);
+}
+
+}  // namespace pad
+
+using namespace pad;
+
+extern "C" {
+
+int pad_kv_append(const pad_kv_cache* cache, const pad_kv_rows* rows, const float* token_weights,
+                  const int32_t* token_positions, void* stream) {
+  const int st = check_rows(cache, rows);
+  if (st != PAD_OK || rows->tokens == 0) return st;
+  if ((cache->positions && !token_positions) || (token_weights && !cache->weights)) return PAD_ERR_NULL_POINTER;
+  RowArgs a = row_args(cache, rows);
+  a.token_weights = token_weights;
+  a.token_positions = token_positions;
+  launch_rows<Append>(a, reinterpret_cast<hipStream_t>(stream));
+  return hipGetLastError() == hipSuccess ? PAD_OK : PAD_ERR_LAUNCH;
+}
+
+int pad_kv_read(const pad_kv_cache* cache, const pad_kv_rows* rows, void* stream) {
+  const int st = check_rows(cache, rows);
+  if (st != PAD_OK || rows->tokens == 0) return st;
+  launch_rows<Read>(row_args(cache, rows), reinterpret_cast<hipStream_t>(stream));
+  return hipGetLastError() == hipSuccess ? PAD_OK : PAD_ERR_LAUNCH;
+}
+
+int pad_kv_evict_workspace_bytes(int64_t batch, int64_t num_kv_heads, int64_t max_pages, int64_t page_size,
+                                 size_t* bytes) {
+  if (!bytes) return PAD_ERR_NULL_POINTER;
+  if (batch < 0 || num_kv_heads <= 0 || max_pages < 0 || page_size <= 0 || max_pages > kMostSlots / page_size)
+    return PAD_ERR_INVALID_SHAPE;
+  *bytes = evict_bytes(batch * num_kv_heads, max_pages, page_size);
+  return PAD_OK;
+}
+
+int pad_kv_evict(const pad_kv_cache* cache, const pad_kv_evict_call* call, void* stream) {
+  int st = check_cache(cache);
+  if (st != PAD_OK) return st;
+  if (!call || !cache->weights || !cache->positions) return PAD_ERR_NULL_POINTER;
+  if (call->batch < 0 || call->batch > 65535 || call->max_pages < 0 || call->recent < 0 ||
+      (!call->keeps && call->keep < 0) || call->max_pages > kMostSlots / cache->page_size)
+    return PAD_ERR_INVALID_SHAPE;
+  if (call->batch == 0) return PAD_OK;
+  if (!call->seq_lens || !call->new_lens || (!call->block_table && call->max_pages > 0)) return PAD_ERR_NULL_POINTER;
+  const int64_t units = (int64_t)call->batch * cache->num_kv_heads;
+  if (!call->workspace || call->workspace_bytes < evict_bytes(units, call->max_pages, cache->page_size))
+    return PAD_ERR_WORKSPACE;
+  EvictArgs a = {};
+  a.c = *cache;
+  a.e = *call;
+  char* base = reinterpret_cast<char*>(((uintptr_t)call->workspace + 255u) & ~(uintptr_t)255u);
+  a.num_moves = reinterpret_cast<int*>(base);
+  a.moves = reinterpret_cast<int2*>(base + evict_counts_bytes(units));
+  a.most = most_moves(call->max_pages, cache->page_size);
+  a.ps_shift = shift_of(cache->page_size);
+  a.elem_bytes = stride_bytes(cache);
+  a.scale_bytes = row_kind(cache->kv_format) == kRowsMx4 ? cache->head_dim / 32 : 0;
+  hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(pad_evict_select_kernel, dim3(cache->num_kv_heads, call->batch), dim3(kEvictThreads), 0, hs, a);
+  if (hipGetLastError() != hipSuccess) return PAD_ERR_LAUNCH;
+  if (a.most == 0) return PAD_OK;
+  const bool wide = row_alignment(cache) == 16;
+  a.row_units = row_bytes(cache) / (wide ? 16 : 8);
+  const int per = 256 / (2 * a.row_units);
+  const int64_t chunks = (a.most + 4 * per - 1) / (4 * per);
+  const int64_t limit = 8192 / units > 1 ? 8192 / units : 1;
+  const dim3 grid((unsigned)(chunks < limit ? chunks : limit), cache->num_kv_heads, call->batch);
+  if (wide)
+    hipLaunchKernelGGL((pad_evict_move_kernel<u4_t>), grid, dim3(256), 0, hs, a);
+  else
+    hipLaunchKernelGGL((pad_evict_move_kernel<u2_t>), grid, dim3(256), 0, hs, a);
+  return hipGetLastError() == hipSuccess ? PAD_OK : PAD_ERR_LAUNCH;
+}
+
+}  // extern "C"

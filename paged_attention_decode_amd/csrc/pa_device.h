@@ -87,6 +87,17 @@ struct Phase1Args {
   int64_t svp, svs, svh;
   int64_t sob, soh;
   int64_t num_pages;
+  // MX4 caches: the scale bytes of K and V (strides in bytes: page, slot, kv
+  // head; a row's blocks are consecutive bytes).
+  const uint8_t* ks;
+  const uint8_t* vs;
+  int64_t sksp, skss, sksh;
+  int64_t svsp, svss, svsh;
+  // kKvWeights: every score in base-2 units, [batch * query heads] rows of
+  // slog floats by token, and log2 of each row's normaliser, [batch * query heads].
+  float* logits;
+  float* lse;
+  int64_t slog;
 #ifdef PAD_TIMELINE
   int tl_launch;   // ring slot of this launch's stamps
 #endif
@@ -399,14 +410,28 @@ constexpr int kKvE5M2 = 2;   // float8_e5m2 caches, fp16 q and output
 constexpr int kKvBF16 = 3;   // bfloat16 q, caches and output
 constexpr int kKvE4M3B = 4;  // float8_e4m3fn caches, bfloat16 q and output
 constexpr int kKvE5M2B = 5;  // float8_e5m2 caches, bfloat16 q and output
+constexpr int kKvMx4 = 6;    // MX4 caches (e2m1 codes, a power-of-two scale per 32), fp16 q and output
+constexpr int kKvMx4B = 7;   // the same, bfloat16 q and output
+constexpr int kKvWeights = 16;  // added to one of these: the call also writes its scores and normalisers
 
 template <int KVF>
-constexpr bool kv_is_fp8() { return KVF == kKvE4M3 || KVF == kKvE5M2 || KVF == kKvE4M3B || KVF == kKvE5M2B; }
+constexpr int kv_base() { return KVF & 15; }
 template <int KVF>
-constexpr bool kv_is_e4m3() { return KVF == kKvE4M3 || KVF == kKvE4M3B; }
+constexpr bool kv_weights() { return (KVF & kKvWeights) != 0; }
+template <int KVF>
+constexpr bool kv_is_mx4() { return kv_base<KVF>() == kKvMx4 || kv_base<KVF>() == kKvMx4B; }
+template <int KVF>
+constexpr bool kv_is_e4m3() { return kv_base<KVF>() == kKvE4M3 || kv_base<KVF>() == kKvE4M3B; }
+template <int KVF>
+constexpr bool kv_is_fp8() {
+  return kv_is_e4m3<KVF>() || kv_base<KVF>() == kKvE5M2 || kv_base<KVF>() == kKvE5M2B;
+}
 // bfloat16 q, P and output (and MFMAs); fp16 otherwise.
 template <int KVF>
-constexpr bool q_is_bf16() { return KVF == kKvBF16 || KVF == kKvE4M3B || KVF == kKvE5M2B; }
+constexpr bool q_is_bf16() {
+  return kv_base<KVF>() == kKvBF16 || kv_base<KVF>() == kKvE4M3B || kv_base<KVF>() == kKvE5M2B ||
+         kv_base<KVF>() == kKvMx4B;
+}
 template <int KVF>
 constexpr int kv_elem_bytes() { return kv_is_fp8<KVF>() ? 1 : 2; }
 

@@ -30,6 +30,7 @@
 #include <utility>
 #include <vector>
 
+#include "pa_cache.h"
 #include "pa_decode.h"
 
 namespace {
@@ -555,6 +556,263 @@ py::dict plan(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t 
   return r;
 }
 
+// ---------------------------------------------------------------------------
+// Cache operators (pa_cache.h; checked by cache.py, which describes them).
+// ---------------------------------------------------------------------------
+using OptTensor = c10::optional<torch::Tensor>;
+
+void check_same_gpu(const torch::Tensor& ref, std::initializer_list<const OptTensor*> others) {
+  TORCH_CHECK(ref.is_cuda(), "pa_decode: all tensors must be on the GPU");
+  for (const OptTensor* t : others)
+    TORCH_CHECK(!t->has_value() || (*t)->device() == ref.device(), "pa_decode: all tensors must be on the same device");
+}
+
+int row_format(const torch::Tensor& cache) {
+  switch (cache.scalar_type()) {
+    case at::kHalf: return PAD_KV_FP16;
+    case at::kBFloat16: return PAD_KV_BF16;
+    case at::kFloat8_e4m3fn: return PAD_KV_FP8_E4M3FN;
+    case at::kFloat8_e5m2: return PAD_KV_FP8_E5M2;
+    case at::kByte: return PAD_KV_MX4;
+    default: TORCH_CHECK(false, "pa_decode: caches must be float16, bfloat16, float8_e4m3fn, float8_e5m2 or uint8");
+  }
+}
+
+void strides3(const torch::Tensor& t, int64_t* out) {
+  for (int i = 0; i < 3; ++i) out[i] = t.stride(i);
+}
+
+// The caches of one layer as the C ABI takes them.
+pad_kv_cache cache_desc(const torch::Tensor& k_cache, const torch::Tensor& v_cache, const OptTensor& k_scales,
+                        const OptTensor& v_scales, const OptTensor& weights, const OptTensor& positions,
+                        double k_scale, double v_scale, int64_t head_dim) {
+  TORCH_CHECK(k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes() &&
+                  v_cache.scalar_type() == k_cache.scalar_type() && k_cache.stride(3) == 1 && v_cache.stride(3) == 1,
+              "pa_decode: the caches must be [num_pages, page_size, num_kv_heads, head_dim], both alike, with a "
+              "contiguous head_dim");
+  check_same_gpu(k_cache, {&k_scales, &v_scales, &weights, &positions});
+  TORCH_CHECK(v_cache.device() == k_cache.device(), "pa_decode: all tensors must be on the same device");
+  pad_kv_cache c;
+  std::memset(&c, 0, sizeof(c));
+  c.kv_format = row_format(k_cache);
+  const int64_t width = c.kv_format == PAD_KV_MX4 ? head_dim / 2 : head_dim;
+  TORCH_CHECK(k_cache.size(3) == width, "pa_decode: head_dim does not match the caches");
+  c.k = k_cache.data_ptr();
+  c.v = v_cache.data_ptr();
+  strides3(k_cache, c.k_stride);
+  strides3(v_cache, c.v_stride);
+  if (c.kv_format == PAD_KV_MX4) {
+    for (const OptTensor* s : {&k_scales, &v_scales})
+      TORCH_CHECK(s->has_value() && (*s)->scalar_type() == at::kByte && (*s)->dim() == 4 &&
+                      (*s)->size(0) == k_cache.size(0) && (*s)->size(1) == k_cache.size(1) &&
+                      (*s)->size(2) == k_cache.size(2) && (*s)->size(3) == head_dim / 32 && (*s)->stride(3) == 1,
+                  "pa_decode: MX4 caches need uint8 scales [num_pages, page_size, num_kv_heads, head_dim / 32]");
+    c.k_scales = k_scales->data_ptr<uint8_t>();
+    c.v_scales = v_scales->data_ptr<uint8_t>();
+    strides3(*k_scales, c.ks_stride);
+    strides3(*v_scales, c.vs_stride);
+  }
+  const auto check_state = [&](const torch::Tensor& t, at::ScalarType type) {
+    TORCH_CHECK(t.scalar_type() == type && t.dim() == 3 && t.size(0) == k_cache.size(0) &&
+                    t.size(1) == k_cache.size(1) && t.size(2) == k_cache.size(2),
+                "pa_decode: weights (float32) and positions (int32) must be [num_pages, page_size, num_kv_heads]");
+  };
+  if (weights.has_value()) {
+    check_state(*weights, at::kFloat);
+    c.weights = weights->data_ptr<float>();
+    strides3(*weights, c.w_stride);
+  }
+  if (positions.has_value()) {
+    check_state(*positions, at::kInt);
+    c.positions = positions->data_ptr<int32_t>();
+    strides3(*positions, c.p_stride);
+  }
+  TORCH_CHECK(k_cache.size(1) <= INT32_MAX && k_cache.size(2) <= INT32_MAX, "pa_decode: cache too large");
+  c.num_pages = k_cache.size(0);
+  c.page_size = static_cast<int32_t>(k_cache.size(1));
+  c.num_kv_heads = static_cast<int32_t>(k_cache.size(2));
+  c.head_dim = static_cast<int32_t>(head_dim);
+  c.k_scale = static_cast<float>(k_scale);
+  c.v_scale = static_cast<float>(v_scale);
+  return c;
+}
+
+pad_kv_rows rows_desc(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& slots) {
+  TORCH_CHECK(k.dim() == 3 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && k.stride(2) == 1 &&
+                  v.stride(2) == 1 && (k.scalar_type() == at::kHalf || k.scalar_type() == at::kBFloat16),
+              "pa_decode: k and v must be float16 or bfloat16 [tokens, num_kv_heads, head_dim], both alike");
+  TORCH_CHECK(slots.dim() == 1 && slots.size(0) == k.size(0) && slots.is_contiguous() &&
+                  (slots.scalar_type() == at::kLong || slots.scalar_type() == at::kInt),
+              "pa_decode: slots must be int32 or int64 [tokens]");
+  TORCH_CHECK(v.device() == k.device() && slots.device() == k.device(),
+              "pa_decode: all tensors must be on the same device");
+  pad_kv_rows r;
+  std::memset(&r, 0, sizeof(r));
+  r.k = k.data_ptr();
+  r.v = v.data_ptr();
+  for (int i = 0; i < 2; ++i) {
+    r.k_stride[i] = k.stride(i);
+    r.v_stride[i] = v.stride(i);
+  }
+  r.slots = slots.data_ptr();
+  r.tokens = k.size(0);
+  r.slots64 = slots.scalar_type() == at::kLong ? 1 : 0;
+  r.bf16 = k.scalar_type() == at::kBFloat16 ? 1 : 0;
+  return r;
+}
+
+hipStream_t current_stream(const torch::Tensor& t) {
+  return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device()).stream();
+}
+
+void kv_append(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor slots,
+               OptTensor k_scales, OptTensor v_scales, double k_scale, double v_scale, OptTensor weights,
+               OptTensor positions, OptTensor token_weights, OptTensor token_positions) {
+  const pad_kv_cache c =
+      cache_desc(k_cache, v_cache, k_scales, v_scales, weights, positions, k_scale, v_scale, k.size(2));
+  const pad_kv_rows r = rows_desc(k, v, slots);
+  check_same_gpu(k_cache, {&token_weights, &token_positions});
+  TORCH_CHECK(k.device() == k_cache.device(), "pa_decode: all tensors must be on the same device");
+  TORCH_CHECK(k.size(1) == k_cache.size(2), "pa_decode: k and v do not match the caches' heads");
+  TORCH_CHECK(!token_weights.has_value() ||
+                  (token_weights->scalar_type() == at::kFloat && token_weights->is_contiguous() &&
+                   token_weights->numel() == k.size(0) * k.size(1)),
+              "pa_decode: token_weights must be contiguous float32 [tokens, num_kv_heads]");
+  TORCH_CHECK(!token_positions.has_value() ||
+                  (token_positions->scalar_type() == at::kInt && token_positions->is_contiguous() &&
+                   token_positions->numel() == k.size(0)),
+              "pa_decode: token_positions must be contiguous int32 [tokens]");
+  if (k.size(0) == 0) return;
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(k.device());
+  const int st = pad_kv_append(&c, &r, token_weights.has_value() ? token_weights->data_ptr<float>() : nullptr,
+                               token_positions.has_value() ? token_positions->data_ptr<int32_t>() : nullptr,
+                               current_stream(k));
+  TORCH_CHECK(st == PAD_OK, "pa_decode: ", pad_status_string(st));
+}
+
+std::tuple<torch::Tensor, torch::Tensor> kv_read(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor slots,
+                                                 OptTensor k_scales, OptTensor v_scales, double k_scale,
+                                                 double v_scale, int64_t head_dim, bool bf16) {
+  const pad_kv_cache c = cache_desc(k_cache, v_cache, k_scales, v_scales, c10::nullopt, c10::nullopt, k_scale, v_scale,
+                                    head_dim);
+  TORCH_CHECK(slots.is_cuda() && slots.dim() == 1, "pa_decode: slots must be a 1-D GPU tensor");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+  const auto options = k_cache.options().dtype(bf16 ? at::kBFloat16 : at::kHalf);
+  auto k = torch::empty({slots.size(0), k_cache.size(2), head_dim}, options);
+  auto v = torch::empty_like(k);
+  const pad_kv_rows r = rows_desc(k, v, slots);
+  if (slots.size(0) > 0) {
+    const int st = pad_kv_read(&c, &r, current_stream(k));
+    TORCH_CHECK(st == PAD_OK, "pa_decode: ", pad_status_string(st));
+  }
+  return {k, v};
+}
+
+torch::Tensor kv_evict(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor weights, torch::Tensor positions,
+                       torch::Tensor block_table, torch::Tensor seq_lens, OptTensor k_scales, OptTensor v_scales,
+                       OptTensor keeps, int64_t keep, int64_t recent, int64_t head_dim) {
+  const pad_kv_cache c = cache_desc(k_cache, v_cache, k_scales, v_scales, weights, positions, 1.0, 1.0, head_dim);
+  const OptTensor bt = block_table, sl = seq_lens;
+  check_same_gpu(k_cache, {&bt, &sl, &keeps});
+  TORCH_CHECK(block_table.scalar_type() == at::kInt && seq_lens.scalar_type() == at::kInt && block_table.dim() == 2 &&
+                  seq_lens.dim() == 1 && block_table.size(0) == seq_lens.size(0),
+              "pa_decode: block_table [batch, max_pages] and seq_lens [batch] must be int32");
+  TORCH_CHECK(!keeps.has_value() || (keeps->scalar_type() == at::kInt && keeps->is_contiguous() &&
+                                     keeps->numel() == seq_lens.size(0)),
+              "pa_decode: keep must be contiguous int32 [batch]");
+  TORCH_CHECK(block_table.size(1) <= INT32_MAX && seq_lens.size(0) <= INT32_MAX && keep >= 0 && keep <= INT32_MAX &&
+                  recent >= 0 && recent <= INT32_MAX,
+              "pa_decode: keep or recent out of range");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+  auto new_lens = torch::empty({seq_lens.size(0)}, seq_lens.options());
+  size_t bytes = 0;
+  int st = pad_kv_evict_workspace_bytes(seq_lens.size(0), c.num_kv_heads, block_table.size(1), c.page_size, &bytes);
+  TORCH_CHECK(st == PAD_OK, "pa_decode: ", pad_status_string(st));
+  auto ws = torch::empty({static_cast<int64_t>(bytes)}, k_cache.options().dtype(at::kByte));
+  pad_kv_evict_call e;
+  std::memset(&e, 0, sizeof(e));
+  e.block_table = block_table.data_ptr<int32_t>();
+  e.seq_lens = seq_lens.data_ptr<int32_t>();
+  e.keeps = keeps.has_value() ? keeps->data_ptr<int32_t>() : nullptr;
+  e.new_lens = new_lens.data_ptr<int32_t>();
+  e.workspace = ws.data_ptr();
+  e.workspace_bytes = bytes;
+  e.bt_stride[0] = block_table.stride(0);
+  e.bt_stride[1] = block_table.stride(1);
+  e.sl_stride = seq_lens.stride(0);
+  e.batch = static_cast<int32_t>(seq_lens.size(0));
+  e.max_pages = static_cast<int32_t>(block_table.size(1));
+  e.keep = static_cast<int32_t>(keep);
+  e.recent = static_cast<int32_t>(recent);
+  st = pad_kv_evict(&c, &e, current_stream(k_cache));
+  TORCH_CHECK(st == PAD_OK, "pa_decode: ", pad_status_string(st));
+  return new_lens;
+}
+
+// Decode over MX4 caches, or with accumulated weights, or both: forward()'s plan,
+// scratch and stream; the scores' scratch comes from PyTorch's allocator.
+torch::Tensor cache_decode(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor block_table,
+                           torch::Tensor seq_lens, OptTensor k_scales, OptTensor v_scales, OptTensor weights,
+                           double scale, double k_scale, double v_scale, int64_t num_splits) {
+  TORCH_CHECK(q.dim() == 3, "pa_decode: q must be [batch, num_q_heads, head_dim]");
+  const pad_kv_cache desc =
+      cache_desc(k_cache, v_cache, k_scales, v_scales, weights, c10::nullopt, k_scale, v_scale, q.size(2));
+  const bool mx4 = desc.kv_format == PAD_KV_MX4;
+  TORCH_CHECK(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16,
+              "pa_decode: q must be float16 or bfloat16");
+  const OptTensor oq = q, bt = block_table, sl = seq_lens;
+  check_same_gpu(k_cache, {&oq, &bt, &sl});
+  TORCH_CHECK(block_table.scalar_type() == at::kInt && seq_lens.scalar_type() == at::kInt && block_table.dim() == 2 &&
+                  seq_lens.dim() == 1 && block_table.size(0) == q.size(0) && seq_lens.size(0) == q.size(0),
+              "pa_decode: block_table [batch, max_pages] and seq_lens [batch] must be int32");
+  TORCH_CHECK(num_splits >= 0 && num_splits <= INT32_MAX, "pa_decode: num_splits out of range");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  auto out = torch::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+  if (q.size(0) == 0) return out;
+  pad_decode_dims d;
+  fill_dims(q, k_cache, v_cache, block_table, seq_lens, out, &d);
+  pad_decode_plan_t plan;
+  const int cus = cached_cus(q.get_device());
+  int st = pad_decode_plan(&d, static_cast<int>(num_splits), cus, &plan);
+  TORCH_CHECK(st == PAD_OK, "pa_decode: ", pad_status_string(st));
+  hipStream_t stream = current_stream(q);
+  pad_cache_call cc;
+  std::memset(&cc, 0, sizeof(cc));
+  pad_decode_call& c = cc.call;
+  c.q = q.data_ptr();
+  c.k_cache = k_cache.data_ptr();
+  c.v_cache = v_cache.data_ptr();
+  c.block_table = block_table.data_ptr<int32_t>();
+  c.seq_lens = seq_lens.data_ptr<int32_t>();
+  c.out = out.data_ptr();
+  const LaunchScratch scratch = launch_scratch(q, stream, d, static_cast<int>(num_splits), cus, false, plan);
+  c.workspace = scratch.workspace;
+  c.workspace_bytes = scratch.workspace_bytes;
+  c.counters = scratch.counters;
+  c.num_counters = scratch.num_counters;
+  c.scale = static_cast<float>(scale);
+  c.num_splits = static_cast<int32_t>(num_splits);
+  c.kv_format = mx4 ? (q.scalar_type() == at::kHalf ? PAD_KV_MX4 : PAD_KV_MX4_BF16) : cache_format(q, k_cache, v_cache);
+  c.k_scale = static_cast<float>(k_scale);
+  c.v_scale = static_cast<float>(v_scale);
+  cc.k_scales = desc.k_scales;
+  cc.v_scales = desc.v_scales;
+  std::memcpy(cc.ks_stride, desc.ks_stride, sizeof(cc.ks_stride));
+  std::memcpy(cc.vs_stride, desc.vs_stride, sizeof(cc.vs_stride));
+  torch::Tensor logits;
+  if (weights.has_value()) {
+    cc.weights = desc.weights;
+    std::memcpy(cc.w_stride, desc.w_stride, sizeof(cc.w_stride));
+    st = pad_cache_logits_bytes(&d, &cc.logits_bytes);
+    TORCH_CHECK(st == PAD_OK, "pa_decode: ", pad_status_string(st));
+    logits = torch::empty({static_cast<int64_t>(cc.logits_bytes)}, q.options().dtype(at::kByte));
+    cc.logits = logits.data_ptr();
+  }
+  st = pad_cache_decode(&cc, &d, stream);
+  TORCH_CHECK(st == PAD_OK, "pa_decode: ", pad_status_string(st));
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -594,5 +852,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("indptr"), py::arg("indices"),
         py::arg("last_page_len"), py::arg("worklist"), py::arg("scale"), py::arg("num_splits"),
         py::arg("k_scale") = 1.0, py::arg("v_scale") = 1.0);
+  m.def("kv_append", &kv_append, "Store rows in a paged cache (see paged_kv_append)");
+  m.def("kv_read", &kv_read, "Rows of a paged cache as values (see paged_kv_read)");
+  m.def("kv_evict", &kv_evict, "Cut sequences to their newest and heaviest tokens (see paged_kv_evict) -> new lengths");
+  m.def("cache_decode", &cache_decode,
+        "Decode over MX4 caches, or with accumulated weights (see paged_attention_decode_mx4, "
+        "paged_attention_decode_weights) -> out");
   m.def("abi_version", &pad_decode_abi_version, "C ABI version of the linked libpa_decode.so");
 }
