@@ -283,26 +283,32 @@ hipError_t launch_accumulate(const Phase1Args& p, float* weights, const int64_t*
 
 // ---------------------------------------------------------------------------
 // Eviction.  Per (sequence, kv head): the keep-th largest key by radix selection
-// (three digits of 11, 11 and 10 bits of an order-preserving integer of the
-// weight), ties by slot order, then the list of moves: the i-th kept slot at or
-// above the new length goes to the i-th evicted slot below it.  Sources lie at or
-// above the new length and targets below it, so no move can overwrite what
-// another reads, and moves run in any order.
+// (four digits of 8 bits of an order-preserving integer of the weight), ties by
+// slot order, then the moves: the i-th kept slot at or above the new length goes
+// to the i-th evicted slot below it.  Sources lie at or above the new length and
+// targets below it, so no move can overwrite what another reads, and moves run
+// in any order.
+//
+// A workgroup selects for one unit; few barriers bound it, so every wave scans
+// the 256 counts of a digit by itself (one barrier a digit), and keys stay in
+// registers: they are read once, a round trip for the page ids and one for
+// weights and positions.
 // ---------------------------------------------------------------------------
 struct EvictArgs {
   pad_kv_cache c;
   pad_kv_evict_call e;
   int2* moves;     // [units][most] (source slot, target slot)
-  int* num_moves;  // [units]
+  int* num_moves;  // [units]: those left to the move kernel
   int64_t most;
   int ps_shift;
   int row_units;   // vector units of a K (or V) row
   int elem_bytes;  // bytes per element of the rows' strides
   int scale_bytes; // MX4 scale bytes of a row, else 0
+  int wide;        // 1: units of 16 bytes, 0: of 8
 };
 
-constexpr int kEvictThreads = 1024;
-constexpr int kEvictWaves = kEvictThreads / 64;
+// Moves that the selecting workgroup makes itself, without a second kernel.
+constexpr int kOwnMoves = 128;
 constexpr uint32_t kKeyNewest = 0xffffffffu;
 constexpr uint32_t kKeyNan = 0xfffffffeu;
 
@@ -317,7 +323,7 @@ __device__ __forceinline__ int evict_page(const EvictArgs& a, int slot) {
   return a.ps_shift >= 0 ? slot >> a.ps_shift : (int)((uint32_t)slot / (uint32_t)a.c.page_size);
 }
 
-// Offset helper: where a slot of sequence b lies.
+// Where a slot of sequence b lies.
 struct Place {
   int64_t page, at;
 };
@@ -329,159 +335,23 @@ __device__ __forceinline__ Place evict_place(const EvictArgs& a, int b, int slot
   return p;
 }
 
-// Exclusive prefix of one count per wave, and their total (every thread calls it).
-__device__ __forceinline__ int wave_base(int count, int wave, int* sm, int& total) {
-  if ((threadIdx.x & 63) == 0) sm[wave] = count;
-  __syncthreads();
-  int base = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kEvictWaves; ++w) {
-    const int c = sm[w];
-    base += w < wave ? c : 0;
-    all += c;
-  }
-  total = all;
-  __syncthreads();
-  return base;
-}
-
-__global__ __launch_bounds__(kEvictThreads) void pad_evict_select_kernel(const EvictArgs a) {
-  const int h = blockIdx.x, b = blockIdx.y;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t unit = (int64_t)b * a.c.num_kv_heads + h;
-  const int64_t cap = (int64_t)a.e.max_pages * a.c.page_size;
-  const int L = (int)min((int64_t)max(a.e.seq_lens[(int64_t)b * a.e.sl_stride], 0), cap);
-  const int n = min(max(a.e.keeps ? a.e.keeps[b] : a.e.keep, 0), L);
-  if (tid == 0 && h == 0) a.e.new_lens[b] = n;
-  if (n == L || n == 0) {
-    if (tid == 0) a.num_moves[unit] = 0;
-    return;
-  }
-  __shared__ int hist[2048];
-  __shared__ int sm[kEvictWaves];
-  __shared__ int s_bin, s_above;
-
-  // A wave has consecutive slots, 64 at a time.
-  const int steps = (L + kEvictThreads - 1) / kEvictThreads;
-  const int first = wave * steps * 64 + lane;
-  auto weight_at = [&](int slot) {
-    const Place p = evict_place(a, b, slot);
-    return a.c.weights[p.page * a.c.w_stride[0] + p.at * a.c.w_stride[1] + (int64_t)h * a.c.w_stride[2]];
-  };
-  auto position_at = [&](int slot) {
-    const Place p = evict_place(a, b, slot);
-    return a.c.positions[p.page * a.c.p_stride[0] + p.at * a.c.p_stride[1] + (int64_t)h * a.c.p_stride[2]];
-  };
-  int newest = INT32_MIN;
-  for (int i = 0; i < steps; ++i) {
-    const int slot = first + i * 64;
-    if (slot < L) newest = max(newest, position_at(slot));
-  }
-  newest = wave_max_i32(newest);
-  if (lane == 0) sm[wave] = newest;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kEvictWaves; ++w) newest = max(newest, sm[w]);
-  __syncthreads();
-  const int64_t border = (int64_t)newest - a.e.recent;
-  auto key_at = [&](int slot) -> uint32_t {
-    if (slot >= L) return 0u;
-    if ((int64_t)position_at(slot) > border) return kKeyNewest;
-    return weight_key(weight_at(slot));
-  };
-
-  // The n-th largest key.
-  uint32_t prefix = 0, mask = 0;
-  int left = n;  // of the keys with this prefix, how many from the top
-#pragma unroll
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const uint32_t bins = pass == 2 ? 1024u : 2048u;
-    for (int i = tid; i < 2048; i += kEvictThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i = 0; i < steps; ++i) {
-      const uint32_t k = key_at(first + i * 64);
-      if (k != 0 && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
-    }
-    __syncthreads();
-    // Thread t has bins 2047 - 2t and the one below: counts from the top.
-    const int hi = hist[2047 - 2 * tid], lo = hist[2046 - 2 * tid];
-    const int incl = wave_incl_scan_i32(hi + lo, lane);
-    int total;
-    const int base = wave_base(__builtin_amdgcn_readlane(incl, 63), wave, sm, total) + incl - hi - lo;
-    if (base < left && left <= base + hi) {
-      s_bin = 2047 - 2 * tid;
-      s_above = base;
-    } else if (base + hi < left && left <= base + hi + lo) {
-      s_bin = 2046 - 2 * tid;
-      s_above = base + hi;
-    }
-    __syncthreads();
-    prefix |= (uint32_t)s_bin << shift;
-    mask |= (bins - 1) << shift;
-    left -= s_above;
-    __syncthreads();
-  }
-  const uint32_t border_key = prefix;
-
-  // `left` of the keys equal to it are kept, the lowest slots first.
-  int ties = 0, total;
-  for (int i = 0; i < steps; ++i)
-    ties += (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key_at(first + i * 64) == border_key));
-  int tie = wave_base(ties, wave, sm, total);
-  const uint64_t below = (1ull << lane) - 1;
-  const int tie0 = tie;
-  int movers = 0, holes = 0;
-  for (int round = 0; round < 2; ++round) {
-    int mover = 0, hole = 0;
-    if (round == 1) {
-      mover = wave_base(movers, wave, sm, total);
-      hole = wave_base(holes, wave, sm, total);
-      tie = tie0;
-    }
-    for (int i = 0; i < steps; ++i) {
-      const int slot = first + i * 64;
-      const uint32_t k = key_at(slot);
-      const uint64_t eq = __builtin_amdgcn_ballot_w64(k == border_key);
-      const bool kept = k > border_key || (k == border_key && tie + (int)__builtin_popcountll(eq & below) < left);
-      tie += (int)__builtin_popcountll(eq);
-      const bool moves = kept && slot >= n, opens = !kept && slot < n;
-      const uint64_t mv = __builtin_amdgcn_ballot_w64(moves), op = __builtin_amdgcn_ballot_w64(opens);
-      if (round == 0) {
-        movers += (int)__builtin_popcountll(mv);
-        holes += (int)__builtin_popcountll(op);
-      } else {
-        int2* list = a.moves + unit * a.most;
-        const int m = mover + (int)__builtin_popcountll(mv & below), o = hole + (int)__builtin_popcountll(op & below);
-        if (moves && m < a.most) list[m].x = slot;
-        if (opens && o < a.most) list[o].y = slot;
-        mover += (int)__builtin_popcountll(mv);
-        hole += (int)__builtin_popcountll(op);
-      }
-    }
-  }
-  if (tid == 0) a.num_moves[unit] = (int)min((int64_t)total, a.most);
-}
-
-// Moves: TP = 2 * row_units threads per move (K's vector units, then V's).
+// Moves first, first + step, ... of m by `threads` threads, 2 * row_units for
+// a move: K's vector units, then V's (the first ones take the scales, weight and
+// position along).
 template <typename U>
-__global__ __launch_bounds__(256) void pad_evict_move_kernel(const EvictArgs a) {
-  const int h = blockIdx.y, b = blockIdx.z;
-  const int64_t unit = (int64_t)b * a.c.num_kv_heads + h;
-  const int m = a.num_moves[unit];
+__device__ __forceinline__ void move_rows(const EvictArgs& a, int b, int h, const int2* list, int m, int block,
+                                          int blocks, int tid, int threads) {
   const int tp = 2 * a.row_units;
-  const int per = 256 / tp;
-  const int mine = threadIdx.x / tp;
+  const int per = threads / tp;
+  const int mine = tid / tp;
   if (mine >= per) return;
-  const int task = threadIdx.x - mine * tp;
+  const int task = tid - mine * tp;
   const bool is_v = task >= a.row_units;
   const int c = is_v ? task - a.row_units : task;
   const int64_t* st = is_v ? a.c.v_stride : a.c.k_stride;
   const int64_t* ss = is_v ? a.c.vs_stride : a.c.ks_stride;
   char* base = static_cast<char*>(is_v ? a.c.v : a.c.k) + (int64_t)h * st[2] * a.elem_bytes + c * sizeof(U);
-  const int2* list = a.moves + unit * a.most;
-  for (int i = blockIdx.x * per + mine; i < m; i += gridDim.x * per) {
+  for (int i = block * per + mine; i < m; i += blocks * per) {
     const int2 mv = list[i];
     const Place s = evict_place(a, b, mv.x), d = evict_place(a, b, mv.y);
     *reinterpret_cast<U*>(base + (d.page * st[0] + d.at * st[1]) * a.elem_bytes) =
@@ -500,6 +370,218 @@ __global__ __launch_bounds__(256) void pad_evict_move_kernel(const EvictArgs a) 
       }
     }
   }
+}
+
+// Adds one to hist[bin] for every lane with `in`: the lanes that share the first
+// one's bin in one addition (weights of a digit fall into few bins).
+__device__ __forceinline__ void count_bin(int* hist, int bin, bool in, int lane) {
+  const uint64_t active = __builtin_amdgcn_ballot_w64(in);
+  if (active == 0) return;
+  const int lead = (int)__builtin_ctzll(active);
+  const int common = __builtin_amdgcn_readlane(bin, lead);
+  const uint64_t same = __builtin_amdgcn_ballot_w64(in && bin == common);
+  if (lane == lead) atomicAdd(&hist[common], (int)__builtin_popcountll(same));
+  if (in && bin != common) atomicAdd(&hist[bin], 1);
+}
+
+// NR: slots of a thread, whose keys are in registers; 0: any number, read again
+// in every pass.
+template <int NR, int THREADS>
+__global__ __launch_bounds__(THREADS) void pad_evict_select_kernel(const EvictArgs a) {
+  constexpr int WAVES = THREADS / 64;
+  const int h = blockIdx.x, b = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t unit = (int64_t)b * a.c.num_kv_heads + h;
+  const int64_t cap = (int64_t)a.e.max_pages * a.c.page_size;
+  const int L = (int)min((int64_t)max(a.e.seq_lens[(int64_t)b * a.e.sl_stride], 0), cap);
+  const int n = min(max(a.e.keeps ? a.e.keeps[b] : a.e.keep, 0), L);
+  if (tid == 0 && h == 0) a.e.new_lens[b] = n;
+  if (n == L || n == 0) {
+    if (tid == 0) a.num_moves[unit] = 0;
+    return;
+  }
+  __shared__ int hist[4][256];
+  __shared__ int sm[2][WAVES];
+  __shared__ int2 own[kOwnMoves];
+  for (int i = tid; i < 4 * 256; i += THREADS) hist[0][i] = 0;
+
+  // A wave has consecutive slots, 64 at a time.
+  const int steps = (L + THREADS - 1) / THREADS;
+  const int first = wave * steps * 64 + lane;
+  const char* wbase = reinterpret_cast<const char*>(a.c.weights + (int64_t)h * a.c.w_stride[2]);
+  const char* pbase = reinterpret_cast<const char*>(a.c.positions + (int64_t)h * a.c.p_stride[2]);
+  auto weight_of = [&](const Place& p) {
+    return *reinterpret_cast<const float*>(wbase + (p.page * a.c.w_stride[0] + p.at * a.c.w_stride[1]) * 4);
+  };
+  auto position_of = [&](const Place& p) {
+    return *reinterpret_cast<const int32_t*>(pbase + (p.page * a.c.p_stride[0] + p.at * a.c.p_stride[1]) * 4);
+  };
+  constexpr int N = NR > 0 ? NR : 1;
+  uint32_t keys[N];
+  int64_t border;
+  {
+    int newest = INT32_MIN;
+    int positions[N];
+    if constexpr (NR > 0) {
+      // Slots past the end read the last one's words (and get key 0 below): no
+      // branch holds a load back.
+      constexpr int BATCH = NR < 8 ? NR : 8;
+#pragma unroll
+      for (int i0 = 0; i0 < NR; i0 += BATCH) {
+        if (i0 < steps) {
+          Place p[BATCH];
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) p[i] = evict_place(a, b, min(first + (i0 + i) * 64, L - 1));
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) {
+            positions[i0 + i] = position_of(p[i]);
+            keys[i0 + i] = __float_as_uint(weight_of(p[i]));
+          }
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) newest = max(newest, positions[i0 + i]);
+        }
+      }
+    } else {
+      for (int i = 0; i < steps; ++i) {
+        const int slot = first + i * 64;
+        if (slot < L) newest = max(newest, position_of(evict_place(a, b, slot)));
+      }
+    }
+    newest = wave_max_i32(newest);
+    if (lane == 0) sm[0][wave] = newest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) newest = max(newest, sm[0][w]);
+    border = (int64_t)newest - a.e.recent;
+    if constexpr (NR > 0) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const bool in = i < steps && first + i * 64 < L;
+        const uint32_t k = (int64_t)positions[i] > border ? kKeyNewest : weight_key(__uint_as_float(keys[i]));
+        keys[i] = in ? k : 0u;
+      }
+    }
+  }
+  auto key_at = [&](int i) -> uint32_t {
+    if constexpr (NR > 0) {
+      return keys[i];
+    } else {
+      const int slot = first + i * 64;
+      if (slot >= L) return 0u;
+      const Place p = evict_place(a, b, slot);
+      const int32_t at = position_of(p);
+      const float w = weight_of(p);
+      return (int64_t)at > border ? kKeyNewest : weight_key(w);
+    }
+  };
+  // f(i, key) for each of the thread's slots; whole waves call it.
+  auto each = [&](auto f) {
+    if constexpr (NR > 0) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+        if (i < steps) f(i, keys[i]);
+    } else {
+      for (int i = 0; i < steps; ++i) f(i, key_at(i));
+    }
+  };
+
+  // The n-th largest key.
+  uint32_t prefix = 0;
+  int left = n;  // of the keys with this prefix, how many from the top
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
+    each([&](int, uint32_t k) {
+      const bool in = k != 0 && (pass == 0 || (k >> (shift + 8)) == (prefix >> (shift + 8)));
+      count_bin(hist[pass], (int)((k >> shift) & 255u), in, lane);
+    });
+    __syncthreads();
+    // Lane l has bins 255 - 4l and the three below, from the top.
+    const i4_t c = *reinterpret_cast<const i4_t*>(&hist[pass][252 - 4 * lane]);
+    const int sum = c[0] + c[1] + c[2] + c[3];
+    int above = wave_incl_scan_i32(sum, lane) - sum;
+    int bin = -1;
+    int above_bin = 0;
+#pragma unroll
+    for (int j = 3; j >= 0; --j) {
+      if (above < left && left <= above + c[j]) {
+        bin = 252 - 4 * lane + j;
+        above_bin = above;
+      }
+      above += c[j];
+    }
+    const int who = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(bin >= 0));  // the keys counted are at least `left`
+    prefix |= (uint32_t)__builtin_amdgcn_readlane(bin, who) << shift;
+    left -= __builtin_amdgcn_readlane(above_bin, who);
+  }
+
+  // `left` of the keys equal to it are kept, the lowest slots first.
+  const uint64_t below = (1ull << lane) - 1;
+  auto counts_before = [&](int count, int* place, int& total) {  // exclusive prefix over the waves
+    if (lane == 0) place[wave] = count;
+    __syncthreads();
+    int base = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const int c = place[w];
+      base += w < wave ? c : 0;
+      total += c;
+    }
+    return base;
+  };
+  int ties = 0, total;
+  each([&](int, uint32_t k) { ties += (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(k == prefix)); });
+  // (Two places in turn: a wave that writes one has passed a barrier that all
+  // reached after reading it.)
+  const int tie0 = counts_before(ties, sm[1], total);
+  int tie = tie0, movers = 0, holes = 0;
+  auto classify = [&](int i, uint32_t k, uint64_t& moves, uint64_t& opens) {
+    const int slot = first + i * 64;
+    const uint64_t eq = __builtin_amdgcn_ballot_w64(k == prefix);
+    const bool kept = k > prefix || (k == prefix && tie + (int)__builtin_popcountll(eq & below) < left);
+    tie += (int)__builtin_popcountll(eq);
+    moves = __builtin_amdgcn_ballot_w64(kept && slot >= n);
+    opens = __builtin_amdgcn_ballot_w64(!kept && slot < n);
+  };
+  each([&](int i, uint32_t k) {
+    uint64_t mv, op;
+    classify(i, k, mv, op);
+    movers += (int)__builtin_popcountll(mv);
+    holes += (int)__builtin_popcountll(op);
+  });
+  int num_moves;
+  int mover = counts_before(movers, sm[0], num_moves);
+  int hole = counts_before(holes, sm[1], total);
+  num_moves = (int)min((int64_t)num_moves, a.most);
+  const bool mine = num_moves <= kOwnMoves;
+  int2* list = mine ? own : a.moves + unit * a.most;
+  tie = tie0;
+  each([&](int i, uint32_t k) {
+    uint64_t mv, op;
+    classify(i, k, mv, op);
+    const int slot = first + i * 64;
+    const int m = mover + (int)__builtin_popcountll(mv & below), o = hole + (int)__builtin_popcountll(op & below);
+    if ((mv >> lane & 1) && m < num_moves) list[m].x = slot;
+    if ((op >> lane & 1) && o < num_moves) list[o].y = slot;
+    mover += (int)__builtin_popcountll(mv);
+    hole += (int)__builtin_popcountll(op);
+  });
+  if (tid == 0) a.num_moves[unit] = mine ? 0 : num_moves;
+  if (!mine) return;
+  __syncthreads();
+  if (a.wide)
+    move_rows<u4_t>(a, b, h, own, num_moves, 0, 1, tid, THREADS);
+  else
+    move_rows<u2_t>(a, b, h, own, num_moves, 0, 1, tid, THREADS);
+}
+
+template <typename U>
+__global__ __launch_bounds__(256) void pad_evict_move_kernel(const EvictArgs a) {
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int64_t unit = (int64_t)b * a.c.num_kv_heads + h;
+  move_rows<U>(a, b, h, a.moves + unit * a.most, a.num_moves[unit], blockIdx.x, gridDim.x, threadIdx.x, 256);
 }
 
 // ---------------------------------------------------------------------------
@@ -608,7 +690,7 @@ static RowArgs row_args(const pad_kv_cache* c, const pad_kv_rows* r) {
 
 // Slots of one sequence: the selection counts them, in steps of a workgroup, in
 // 32 bits.
-constexpr int64_t kMostSlots = INT32_MAX - 2 * kEvictThreads;
+constexpr int64_t kMostSlots = INT32_MAX - 2 * 1024;
 
 // Workspace of an eviction: 256 bytes of slack, a count per unit, the move lists.  A unit of
 // capacity C moves at most C / 2 rows (sources at or above the new length,
@@ -617,6 +699,23 @@ static int64_t most_moves(int64_t max_pages, int64_t page_size) { return max_pag
 static size_t evict_counts_bytes(int64_t units) { return ((size_t)units * sizeof(int) + 255) & ~(size_t)255; }
 static size_t evict_bytes(int64_t units, int64_t max_pages, int64_t page_size) {
   return 256 + evict_counts_bytes(units) + (size_t)(units * most_moves(max_pages, page_size)) * sizeof(int2);
+}
+
+static void launch_select(const EvictArgs& a, hipStream_t st) {
+  const dim3 grid(a.c.num_kv_heads, a.e.batch);
+  const int64_t cap = (int64_t)a.e.max_pages * a.c.page_size;
+  if (cap <= 2 * 1024)
+    hipLaunchKernelGGL((pad_evict_select_kernel<2, 1024>), grid, dim3(1024), 0, st, a);
+  else if (cap <= 4 * 1024)
+    hipLaunchKernelGGL((pad_evict_select_kernel<4, 1024>), grid, dim3(1024), 0, st, a);
+  else if (cap <= 8 * 1024)
+    hipLaunchKernelGGL((pad_evict_select_kernel<8, 1024>), grid, dim3(1024), 0, st, a);
+  else if (cap <= 16 * 1024)
+    hipLaunchKernelGGL((pad_evict_select_kernel<16, 1024>), grid, dim3(1024), 0, st, a);
+  else if (cap <= 32 * 1024)
+    hipLaunchKernelGGL((pad_evict_select_kernel<32, 1024>), grid, dim3(1024), 0, st, a);
+  else
+    hipLaunchKernelGGL((pad_evict_select_kernel<0, 1024>), grid, dim3(1024), 0, st, a);
 }
 
 }  // namespace pad
@@ -676,16 +775,21 @@ int pad_kv_evict(const pad_kv_cache* cache, const pad_kv_evict_call* call, void*
   a.elem_bytes = stride_bytes(cache);
   a.scale_bytes = row_kind(cache->kv_format) == kRowsMx4 ? cache->head_dim / 32 : 0;
   hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(pad_evict_select_kernel, dim3(cache->num_kv_heads, call->batch), dim3(kEvictThreads), 0, hs, a);
+  a.wide = row_alignment(cache) == 16 ? 1 : 0;
+  a.row_units = row_bytes(cache) / (a.wide ? 16 : 8);
+  launch_select(a, hs);
   if (hipGetLastError() != hipSuccess) return PAD_ERR_LAUNCH;
-  if (a.most == 0) return PAD_OK;
-  const bool wide = row_alignment(cache) == 16;
-  a.row_units = row_bytes(cache) / (wide ? 16 : 8);
+  // No unit moves more rows than it loses, or than it keeps.
+  const int64_t cap = (int64_t)call->max_pages * cache->page_size;
+  const int64_t bound = call->keeps || call->keep >= cap ? a.most
+                        : cap - call->keep < call->keep  ? cap - call->keep
+                                                         : call->keep;
+  if (bound <= kOwnMoves) return PAD_OK;
   const int per = 256 / (2 * a.row_units);
-  const int64_t chunks = (a.most + 4 * per - 1) / (4 * per);
+  const int64_t chunks = (bound + 4 * per - 1) / (4 * per);
   const int64_t limit = 8192 / units > 1 ? 8192 / units : 1;
   const dim3 grid((unsigned)(chunks < limit ? chunks : limit), cache->num_kv_heads, call->batch);
-  if (wide)
+  if (a.wide)
     hipLaunchKernelGGL((pad_evict_move_kernel<u4_t>), grid, dim3(256), 0, hs, a);
   else
     hipLaunchKernelGGL((pad_evict_move_kernel<u2_t>), grid, dim3(256), 0, hs, a);
