@@ -20,7 +20,8 @@ other within a page, which the kernels read best; any strides with a contiguous
 last axis are taken.
 
 Argument problems visible from metadata raise AssertionError, as in the decode
-operators; the native layer raises RuntimeError.  Nothing reads tensor values on
+operators (the binding checks them: in Python that took longer than a small
+call's kernels); others raise RuntimeError.  Nothing reads tensor values on
 the host: a call never synchronises, runs on the current stream and can be
 captured into a HIP graph.  The reference has no counterparts; its caches are
 fp16 and filled by the caller (tests/kernel_test_utils.py).
@@ -28,17 +29,11 @@ fp16 and filled by the caller (tests/kernel_test_utils.py).
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from ._native import ext
-from .ops import ENGINE_MFMA, FP8_CACHE_DTYPES, MAX_GQA, SUPPORTED_HEAD_DIMS, _aligned_q, _cache_format
 
 MX4_HEAD_DIMS = (64, 128, 256)
-_ROW_DTYPES = (torch.float16, torch.bfloat16)
-_CODE_DTYPES = (torch.uint8, torch.float4_e2m1fn_x2)
-_SCALE_DTYPES = (torch.uint8, torch.float8_e8m0fnu)
 
 
 def mx4_cache(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, device="cuda"):
@@ -54,90 +49,6 @@ def kv_weights(num_pages: int, page_size: int, num_kv_heads: int, device="cuda")
     shape = (num_pages, num_kv_heads, page_size)
     return (torch.zeros(shape, dtype=torch.float32, device=device).transpose(1, 2),
             torch.zeros(shape, dtype=torch.int32, device=device).transpose(1, 2))
-
-
-def _disjoint(t):
-    """No two elements in one place, as far as strides of 0 show it."""
-    return all(s != 0 or n <= 1 for s, n in zip(t.stride(), t.shape))
-
-
-def _is_mx4(cache):
-    return cache.dtype in _CODE_DTYPES
-
-
-def _check_caches(k_cache, v_cache, k_scale, v_scale):
-    """(codes or rows of K, of V, MX4 scales of K, of V, fp8 scales, head_dim) of a pair of caches."""
-    assert k_cache.is_cuda and v_cache.is_cuda, "the caches must be GPU tensors"
-    assert k_cache.dim() == 4 and v_cache.shape == k_cache.shape, (
-        "the caches must be [num_pages, page_size, num_kv_heads, head_dim], both alike"
-    )
-    assert k_cache.dtype == v_cache.dtype, "k_cache and v_cache must have the same dtype"
-    assert k_cache.stride(3) == 1 and v_cache.stride(3) == 1, "K/V caches need a contiguous head_dim"
-    if not _is_mx4(k_cache):
-        assert k_cache.dtype in _ROW_DTYPES + FP8_CACHE_DTYPES, (
-            "caches must be float16, bfloat16, float8_e4m3fn, float8_e5m2 or MX4 codes (uint8)"
-        )
-        head_dim = k_cache.shape[3]
-        if k_cache.dtype in FP8_CACHE_DTYPES:
-            assert head_dim in MX4_HEAD_DIMS, f"fp8 caches: head_dim must be one of {MX4_HEAD_DIMS}"
-            ks = 1.0 if k_scale is None else k_scale
-            vs = 1.0 if v_scale is None else v_scale
-            assert not isinstance(ks, torch.Tensor) and not isinstance(vs, torch.Tensor), (
-                "fp8 caches take per-tensor scales, Python floats"
-            )
-            ks, vs = float(ks), float(vs)
-            assert ks > 0 and vs > 0 and math.isfinite(ks) and math.isfinite(vs), (
-                "k_scale and v_scale must be finite and positive"
-            )
-            return k_cache, v_cache, None, None, ks, vs, head_dim
-        assert head_dim in SUPPORTED_HEAD_DIMS, f"head_dim must be one of {SUPPORTED_HEAD_DIMS}"
-        assert not isinstance(k_scale, torch.Tensor) and not isinstance(v_scale, torch.Tensor) and (
-            k_scale in (None, 1.0) and v_scale in (None, 1.0)
-        ), "k_scale / v_scale apply to fp8 and MX4 caches only"
-        return k_cache, v_cache, None, None, 1.0, 1.0, head_dim
-    head_dim = 2 * k_cache.shape[3]
-    assert head_dim in MX4_HEAD_DIMS, f"MX4 caches: head_dim must be one of {MX4_HEAD_DIMS}"
-    for s in (k_scale, v_scale):
-        assert isinstance(s, torch.Tensor) and s.dtype in _SCALE_DTYPES, "MX4 caches need uint8 scale tensors"
-        assert s.is_cuda and tuple(s.shape) == (*k_cache.shape[:3], head_dim // 32), (
-            "MX4 scales must be [num_pages, page_size, num_kv_heads, head_dim // 32] on the GPU"
-        )
-        assert s.stride(3) == 1, "MX4 scales need a contiguous last axis"
-    return (k_cache.view(torch.uint8), v_cache.view(torch.uint8), k_scale.view(torch.uint8),
-            v_scale.view(torch.uint8), 1.0, 1.0, head_dim)
-
-
-def _check_state(t, k_cache, dtype, name):
-    assert t.is_cuda and t.dtype == dtype and tuple(t.shape) == tuple(k_cache.shape[:3]), (
-        f"{name} must be {dtype} [num_pages, page_size, num_kv_heads] on the GPU"
-    )
-    assert _disjoint(t), f"{name} must not be an expanded tensor"
-
-
-def _check_index(block_table, seq_lens, batch=None):
-    assert block_table.is_cuda and seq_lens.is_cuda, "block_table and seq_lens must be GPU tensors"
-    assert block_table.dim() == 2 and seq_lens.dim() == 1 and seq_lens.shape[0] == block_table.shape[0], (
-        "block_table must be [batch, max_pages] and seq_lens [batch]"
-    )
-    assert batch is None or block_table.shape[0] == batch, "block_table must be [batch, max_pages]"
-    for t in (block_table, seq_lens):
-        assert t.dtype in (torch.int32, torch.int64), "block_table and seq_lens must be int32 or int64"
-    return block_table.to(torch.int32), seq_lens.to(torch.int32)
-
-
-def _check_slots(slots, tokens):
-    assert slots.is_cuda and slots.dim() == 1 and slots.dtype in (torch.int32, torch.int64), (
-        "slots must be a 1-D int32 or int64 GPU tensor"
-    )
-    assert tokens is None or slots.shape[0] == tokens, "slots must name one slot per row"
-    return slots.contiguous()
-
-
-def _aligned_rows(x):
-    """16-byte rows, as the kernels need; copied if they are not."""
-    if x.stride(2) != 1 or x.stride(1) % 8 or x.stride(0) % 8 or x.data_ptr() % 16:
-        return x.contiguous()
-    return x
 
 
 def paged_kv_append(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None, weights=None, positions=None,
@@ -160,34 +71,8 @@ def paged_kv_append(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None, w
     num_kv_heads]``; 0 by default) and to ``token_positions`` (int32 ``[tokens]``,
     required with ``positions``).
     """
-    kc, vc, ks, vs, ksc, vsc, head_dim = _check_caches(k_cache, v_cache, k_scale, v_scale)
-    assert k.is_cuda and v.is_cuda, "k and v must be GPU tensors"
-    assert k.dtype in _ROW_DTYPES and v.dtype == k.dtype, "k and v must both be float16 or both bfloat16"
-    assert k.dim() == 3 and v.shape == k.shape and tuple(k.shape[1:]) == (k_cache.shape[2], head_dim), (
-        "k and v must be [tokens, num_kv_heads, head_dim] of the caches"
-    )
-    assert k_cache.dtype not in _ROW_DTYPES or k_cache.dtype == k.dtype, "16-bit caches take rows of their own type"
-    assert all(_disjoint(t) for t in (kc, vc, ks, vs) if t is not None), "the caches must not be expanded tensors"
-    slots = _check_slots(slots, k.shape[0])
-    if weights is not None:
-        _check_state(weights, k_cache, torch.float32, "weights")
-    if positions is not None:
-        _check_state(positions, k_cache, torch.int32, "positions")
-        assert token_positions is not None, "positions need token_positions"
-    if token_weights is not None:
-        assert weights is not None, "token_weights need weights"
-        assert token_weights.is_cuda and token_weights.dtype == torch.float32 and (
-            tuple(token_weights.shape) == tuple(k.shape[:2])
-        ), "token_weights must be float32 [tokens, num_kv_heads] on the GPU"
-        token_weights = token_weights.contiguous()
-    if token_positions is not None:
-        assert positions is not None, "token_positions need positions"
-        assert token_positions.is_cuda and token_positions.dtype in (torch.int32, torch.int64) and (
-            tuple(token_positions.shape) == tuple(k.shape[:1])
-        ), "token_positions must be int32 or int64 [tokens] on the GPU"
-        token_positions = token_positions.to(torch.int32).contiguous()
-    ext().kv_append(_aligned_rows(k), _aligned_rows(v), kc, vc, slots, ks, vs, ksc, vsc, weights, positions,
-                    token_weights, token_positions)
+    ext().kv_append(k, v, k_cache, v_cache, slots, k_scale, v_scale, weights, positions, token_weights,
+                    token_positions)
 
 
 def paged_kv_read(k_cache, v_cache, slots, k_scale=None, v_scale=None, dtype=None):
@@ -199,33 +84,7 @@ def paged_kv_read(k_cache, v_cache, slots, k_scale=None, v_scale=None, dtype=Non
     bfloat16's range is exact in bfloat16).  A negative slot, or one outside the
     cache, gives zeros.
     """
-    kc, vc, ks, vs, ksc, vsc, head_dim = _check_caches(k_cache, v_cache, k_scale, v_scale)
-    if dtype is None:
-        dtype = k_cache.dtype if k_cache.dtype in _ROW_DTYPES else torch.float16
-    assert dtype in _ROW_DTYPES, "dtype must be float16 or bfloat16"
-    assert k_cache.dtype not in _ROW_DTYPES or k_cache.dtype == dtype, "16-bit caches are read in their own type"
-    return ext().kv_read(kc, vc, _check_slots(slots, None), ks, vs, ksc, vsc, head_dim, dtype == torch.bfloat16)
-
-
-def _decode(q, k_cache, v_cache, block_table, seq_lens, num_splits, scale, k_scale, v_scale, weights):
-    assert q.is_cuda and q.dtype in _ROW_DTYPES, "q must be a float16 or bfloat16 GPU tensor"
-    assert q.dim() == 3, "q must be [batch, num_q_heads, head_dim]"
-    kc, vc, ks, vs, ksc, vsc, head_dim = _check_caches(k_cache, v_cache, k_scale, v_scale)
-    batch, num_q_heads = q.shape[:2]
-    num_kv_heads = k_cache.shape[2]
-    assert q.shape[2] == head_dim, "q head_dim must match the KV cache head_dim"
-    assert num_kv_heads > 0 and num_q_heads % num_kv_heads == 0, (
-        "num_q_heads must be divisible by num_kv_heads (GQA)"
-    )
-    assert num_q_heads // num_kv_heads <= MAX_GQA, f"GQA group larger than {MAX_GQA}"
-    if ks is None:
-        _cache_format(q, k_cache, v_cache, head_dim, ENGINE_MFMA, k_scale, v_scale)
-    block_table, seq_lens = _check_index(block_table, seq_lens, batch)
-    num_splits = 0 if num_splits is None else int(num_splits)
-    assert num_splits >= 0, "num_splits must be >= 1"
-    scale = float(scale) if scale is not None else 1.0 / math.sqrt(head_dim)
-    return ext().cache_decode(_aligned_q(q), kc, vc, block_table, seq_lens, ks, vs, weights, scale, ksc, vsc,
-                              num_splits)
+    return ext().kv_read(k_cache, v_cache, slots, k_scale, v_scale, dtype)
 
 
 def paged_attention_decode_mx4(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, num_splits=None,
@@ -238,9 +97,7 @@ def paged_attention_decode_mx4(q, k_cache, v_cache, k_scale, v_scale, block_tabl
     as q's type holds them.  head_dim 64, 128 or 256, any page size, groups of up
     to 16 query heads.
     """
-    assert _is_mx4(k_cache), "MX4 caches are uint8 (or float4_e2m1fn_x2) codes"
-    assert num_splits is None or int(num_splits) >= 1, "num_splits must be >= 1"
-    return _decode(q, k_cache, v_cache, block_table, seq_lens, num_splits, scale, k_scale, v_scale, None)
+    return ext().cache_decode(q, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, None, scale, num_splits)
 
 
 def paged_attention_decode_weights(q, k_cache, v_cache, weights, block_table, seq_lens, num_splits=None, scale=None,
@@ -257,10 +114,8 @@ def paged_attention_decode_weights(q, k_cache, v_cache, weights, block_table, se
     A page must belong to one sequence of the call: of two that share one, either's
     weights may be lost.
     """
-    assert num_splits is None or int(num_splits) >= 1, "num_splits must be >= 1"
-    assert k_cache.dim() == 4, "bad cache shapes"
-    _check_state(weights, k_cache, torch.float32, "weights")
-    return _decode(q, k_cache, v_cache, block_table, seq_lens, num_splits, scale, k_scale, v_scale, weights)
+    assert weights is not None, "weights must be a float32 tensor"
+    return ext().cache_decode(q, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, weights, scale, num_splits)
 
 
 def paged_kv_evict(k_cache, v_cache, weights, positions, block_table, seq_lens, keep, recent: int = 0, k_scale=None,
@@ -282,20 +137,4 @@ def paged_kv_evict(k_cache, v_cache, weights, positions, block_table, seq_lens, 
     needs no scales here; MX4 passes the scale tensors, which move too).  A page
     must belong to one sequence of the call.
     """
-    kc, vc, ks, vs, _, _, head_dim = _check_caches(k_cache, v_cache, k_scale, v_scale)
-    assert all(_disjoint(t) for t in (kc, vc, ks, vs) if t is not None), "the caches must not be expanded tensors"
-    _check_state(weights, k_cache, torch.float32, "weights")
-    _check_state(positions, k_cache, torch.int32, "positions")
-    block_table, seq_lens = _check_index(block_table, seq_lens)
-    recent = int(recent)
-    assert 0 <= recent < 2**31, "recent must be at least 0"
-    keeps = None
-    if isinstance(keep, torch.Tensor):
-        assert keep.is_cuda and keep.dtype in (torch.int32, torch.int64) and keep.shape == seq_lens.shape, (
-            "keep must be an int, or int32 [batch] on the GPU"
-        )
-        keeps, keep = keep.to(torch.int32).contiguous(), 0
-    else:
-        keep = int(keep)
-        assert 1 <= keep < 2**31, "keep must be at least 1"
-    return ext().kv_evict(kc, vc, weights, positions, block_table, seq_lens, ks, vs, keeps, keep, recent, head_dim)
+    return ext().kv_evict(k_cache, v_cache, weights, positions, block_table, seq_lens, keep, recent, k_scale, v_scale)

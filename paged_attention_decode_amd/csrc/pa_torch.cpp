@@ -23,6 +23,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdint>
 #include <cstring>
 #include <map>
@@ -557,95 +558,179 @@ py::dict plan(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t 
 }
 
 // ---------------------------------------------------------------------------
-// Cache operators (pa_cache.h; checked by cache.py, which describes them).
+// Cache operators (pa_cache.h; cache.py documents them).  Their arguments are
+// checked here rather than in Python, where the checks took longer than the
+// kernels of a small call; what is visible from metadata raises AssertionError
+// all the same, as the decode operators' checks do.
 // ---------------------------------------------------------------------------
 using OptTensor = c10::optional<torch::Tensor>;
 
-void check_same_gpu(const torch::Tensor& ref, std::initializer_list<const OptTensor*> others) {
-  TORCH_CHECK(ref.is_cuda(), "pa_decode: all tensors must be on the GPU");
-  for (const OptTensor* t : others)
-    TORCH_CHECK(!t->has_value() || (*t)->device() == ref.device(), "pa_decode: all tensors must be on the same device");
+#define PAD_ASSERT(cond, msg)                          \
+  do {                                                 \
+    if (!(cond)) {                                     \
+      PyErr_SetString(PyExc_AssertionError, msg);      \
+      throw py::error_already_set();                   \
+    }                                                  \
+  } while (0)
+
+bool is_row_type(const torch::Tensor& t) {
+  return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16;
 }
 
-int row_format(const torch::Tensor& cache) {
-  switch (cache.scalar_type()) {
-    case at::kHalf: return PAD_KV_FP16;
-    case at::kBFloat16: return PAD_KV_BF16;
-    case at::kFloat8_e4m3fn: return PAD_KV_FP8_E4M3FN;
-    case at::kFloat8_e5m2: return PAD_KV_FP8_E5M2;
-    case at::kByte: return PAD_KV_MX4;
-    default: TORCH_CHECK(false, "pa_decode: caches must be float16, bfloat16, float8_e4m3fn, float8_e5m2 or uint8");
-  }
+// No two elements in one place, as far as strides of 0 show it.
+bool disjoint(const torch::Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.stride(i) == 0 && t.size(i) > 1) return false;
+  return true;
 }
 
 void strides3(const torch::Tensor& t, int64_t* out) {
   for (int i = 0; i < 3; ++i) out[i] = t.stride(i);
 }
 
+// A cache's scale argument: an MX4 scale tensor, or a float of fp8 caches.
+struct ScaleArg {
+  OptTensor tensor;
+  double value = 1.0;
+  bool given = false;
+};
+
+ScaleArg scale_arg(const py::object& o) {
+  ScaleArg s;
+  if (o.is_none()) return s;
+  s.given = true;
+  if (THPVariable_Check(o.ptr()))
+    s.tensor = THPVariable_Unpack(o.ptr());
+  else
+    s.value = py::cast<double>(o);
+  return s;
+}
+
 // The caches of one layer as the C ABI takes them.
-pad_kv_cache cache_desc(const torch::Tensor& k_cache, const torch::Tensor& v_cache, const OptTensor& k_scales,
-                        const OptTensor& v_scales, const OptTensor& weights, const OptTensor& positions,
-                        double k_scale, double v_scale, int64_t head_dim) {
-  TORCH_CHECK(k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes() &&
-                  v_cache.scalar_type() == k_cache.scalar_type() && k_cache.stride(3) == 1 && v_cache.stride(3) == 1,
-              "pa_decode: the caches must be [num_pages, page_size, num_kv_heads, head_dim], both alike, with a "
-              "contiguous head_dim");
-  check_same_gpu(k_cache, {&k_scales, &v_scales, &weights, &positions});
+pad_kv_cache cache_desc(const torch::Tensor& k_cache, const torch::Tensor& v_cache, const py::object& k_scale,
+                        const py::object& v_scale) {
+  PAD_ASSERT(k_cache.is_cuda() && v_cache.is_cuda(), "the caches must be GPU tensors");
+  PAD_ASSERT(k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes(),
+             "the caches must be [num_pages, page_size, num_kv_heads, head_dim], both alike");
+  PAD_ASSERT(k_cache.scalar_type() == v_cache.scalar_type(), "k_cache and v_cache must have the same dtype");
+  PAD_ASSERT(k_cache.stride(3) == 1 && v_cache.stride(3) == 1, "K/V caches need a contiguous head_dim");
   TORCH_CHECK(v_cache.device() == k_cache.device(), "pa_decode: all tensors must be on the same device");
+  PAD_ASSERT(k_cache.size(1) > 0 && k_cache.size(2) > 0 && k_cache.size(1) <= INT32_MAX && k_cache.size(2) <= INT32_MAX,
+             "bad cache shapes");
   pad_kv_cache c;
   std::memset(&c, 0, sizeof(c));
-  c.kv_format = row_format(k_cache);
-  const int64_t width = c.kv_format == PAD_KV_MX4 ? head_dim / 2 : head_dim;
-  TORCH_CHECK(k_cache.size(3) == width, "pa_decode: head_dim does not match the caches");
+  int64_t head_dim = k_cache.size(3);
+  bool fp8 = false;
+  switch (k_cache.scalar_type()) {
+    case at::kHalf: c.kv_format = PAD_KV_FP16; break;
+    case at::kBFloat16: c.kv_format = PAD_KV_BF16; break;
+    case at::kFloat8_e4m3fn: c.kv_format = PAD_KV_FP8_E4M3FN; fp8 = true; break;
+    case at::kFloat8_e5m2: c.kv_format = PAD_KV_FP8_E5M2; fp8 = true; break;
+    case at::kByte:
+    case at::kFloat4_e2m1fn_x2: c.kv_format = PAD_KV_MX4; head_dim *= 2; break;
+    default:
+      PAD_ASSERT(false, "caches must be float16, bfloat16, float8_e4m3fn, float8_e5m2 or MX4 codes (uint8)");
+  }
+  const ScaleArg ks = scale_arg(k_scale), vs = scale_arg(v_scale);
+  c.k_scale = c.v_scale = 1.0f;
+  if (c.kv_format == PAD_KV_MX4) {
+    PAD_ASSERT(head_dim == 64 || head_dim == 128 || head_dim == 256, "MX4 caches: head_dim must be 64, 128 or 256");
+    for (const ScaleArg* s : {&ks, &vs}) {
+      PAD_ASSERT(s->tensor.has_value() && (s->tensor->scalar_type() == at::kByte ||
+                                           s->tensor->scalar_type() == at::kFloat8_e8m0fnu),
+                 "MX4 caches need uint8 scale tensors");
+      const torch::Tensor& t = *s->tensor;
+      PAD_ASSERT(t.is_cuda() && t.dim() == 4 && t.size(0) == k_cache.size(0) && t.size(1) == k_cache.size(1) &&
+                     t.size(2) == k_cache.size(2) && t.size(3) == head_dim / 32 && t.stride(3) == 1,
+                 "MX4 scales must be [num_pages, page_size, num_kv_heads, head_dim // 32] on the GPU, the last axis "
+                 "contiguous");
+      TORCH_CHECK(t.device() == k_cache.device(), "pa_decode: all tensors must be on the same device");
+    }
+    c.k_scales = static_cast<uint8_t*>(ks.tensor->data_ptr());
+    c.v_scales = static_cast<uint8_t*>(vs.tensor->data_ptr());
+    strides3(*ks.tensor, c.ks_stride);
+    strides3(*vs.tensor, c.vs_stride);
+  } else {
+    PAD_ASSERT(!ks.tensor.has_value() && !vs.tensor.has_value(), "scale tensors apply to MX4 caches only");
+    if (fp8) {
+      PAD_ASSERT(head_dim == 64 || head_dim == 128 || head_dim == 256, "fp8 caches: head_dim must be 64, 128 or 256");
+      PAD_ASSERT(ks.value > 0 && vs.value > 0 && std::isfinite(ks.value) && std::isfinite(vs.value),
+                 "k_scale and v_scale must be finite and positive");
+      c.k_scale = static_cast<float>(ks.value);
+      c.v_scale = static_cast<float>(vs.value);
+    } else {
+      PAD_ASSERT(head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 256,
+                 "head_dim must be one of (32, 64, 96, 128, 256)");
+      PAD_ASSERT(ks.value == 1.0 && vs.value == 1.0, "k_scale / v_scale apply to fp8 and MX4 caches only");
+    }
+  }
   c.k = k_cache.data_ptr();
   c.v = v_cache.data_ptr();
   strides3(k_cache, c.k_stride);
   strides3(v_cache, c.v_stride);
-  if (c.kv_format == PAD_KV_MX4) {
-    for (const OptTensor* s : {&k_scales, &v_scales})
-      TORCH_CHECK(s->has_value() && (*s)->scalar_type() == at::kByte && (*s)->dim() == 4 &&
-                      (*s)->size(0) == k_cache.size(0) && (*s)->size(1) == k_cache.size(1) &&
-                      (*s)->size(2) == k_cache.size(2) && (*s)->size(3) == head_dim / 32 && (*s)->stride(3) == 1,
-                  "pa_decode: MX4 caches need uint8 scales [num_pages, page_size, num_kv_heads, head_dim / 32]");
-    c.k_scales = k_scales->data_ptr<uint8_t>();
-    c.v_scales = v_scales->data_ptr<uint8_t>();
-    strides3(*k_scales, c.ks_stride);
-    strides3(*v_scales, c.vs_stride);
-  }
-  const auto check_state = [&](const torch::Tensor& t, at::ScalarType type) {
-    TORCH_CHECK(t.scalar_type() == type && t.dim() == 3 && t.size(0) == k_cache.size(0) &&
-                    t.size(1) == k_cache.size(1) && t.size(2) == k_cache.size(2),
-                "pa_decode: weights (float32) and positions (int32) must be [num_pages, page_size, num_kv_heads]");
-  };
-  if (weights.has_value()) {
-    check_state(*weights, at::kFloat);
-    c.weights = weights->data_ptr<float>();
-    strides3(*weights, c.w_stride);
-  }
-  if (positions.has_value()) {
-    check_state(*positions, at::kInt);
-    c.positions = positions->data_ptr<int32_t>();
-    strides3(*positions, c.p_stride);
-  }
-  TORCH_CHECK(k_cache.size(1) <= INT32_MAX && k_cache.size(2) <= INT32_MAX, "pa_decode: cache too large");
   c.num_pages = k_cache.size(0);
   c.page_size = static_cast<int32_t>(k_cache.size(1));
   c.num_kv_heads = static_cast<int32_t>(k_cache.size(2));
   c.head_dim = static_cast<int32_t>(head_dim);
-  c.k_scale = static_cast<float>(k_scale);
-  c.v_scale = static_cast<float>(v_scale);
   return c;
 }
 
-pad_kv_rows rows_desc(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& slots) {
-  TORCH_CHECK(k.dim() == 3 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && k.stride(2) == 1 &&
-                  v.stride(2) == 1 && (k.scalar_type() == at::kHalf || k.scalar_type() == at::kBFloat16),
-              "pa_decode: k and v must be float16 or bfloat16 [tokens, num_kv_heads, head_dim], both alike");
-  TORCH_CHECK(slots.dim() == 1 && slots.size(0) == k.size(0) && slots.is_contiguous() &&
-                  (slots.scalar_type() == at::kLong || slots.scalar_type() == at::kInt),
-              "pa_decode: slots must be int32 or int64 [tokens]");
-  TORCH_CHECK(v.device() == k.device() && slots.device() == k.device(),
+// A call that writes to the caches needs every row in a place of its own.
+void check_written(const torch::Tensor& k_cache, const torch::Tensor& v_cache, const py::object& k_scale,
+                   const py::object& v_scale) {
+  bool ok = disjoint(k_cache) && disjoint(v_cache);
+  for (const py::object* o : {&k_scale, &v_scale})
+    if (THPVariable_Check(o->ptr())) ok = ok && disjoint(THPVariable_Unpack(o->ptr()));
+  PAD_ASSERT(ok, "the caches must not be expanded tensors");
+}
+
+void add_state(pad_kv_cache* c, const torch::Tensor& k_cache, const OptTensor& weights, const OptTensor& positions) {
+  for (const OptTensor* o : {&weights, &positions}) {
+    if (!o->has_value()) continue;
+    const torch::Tensor& t = **o;
+    PAD_ASSERT(t.is_cuda() && t.scalar_type() == (o == &weights ? at::kFloat : at::kInt) && t.dim() == 3 &&
+                   t.size(0) == k_cache.size(0) && t.size(1) == k_cache.size(1) && t.size(2) == k_cache.size(2),
+               "weights (float32) and positions (int32) must be [num_pages, page_size, num_kv_heads] on the GPU");
+    PAD_ASSERT(disjoint(t), "weights and positions must not be expanded tensors");
+    TORCH_CHECK(t.device() == k_cache.device(), "pa_decode: all tensors must be on the same device");
+  }
+  if (weights.has_value()) {
+    c->weights = weights->data_ptr<float>();
+    strides3(*weights, c->w_stride);
+  }
+  if (positions.has_value()) {
+    c->positions = positions->data_ptr<int32_t>();
+    strides3(*positions, c->p_stride);
+  }
+}
+
+torch::Tensor as_int32(const torch::Tensor& t) { return t.scalar_type() == at::kInt ? t : t.to(at::kInt); }
+bool is_index(const torch::Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
+
+torch::Tensor check_slots(const torch::Tensor& slots, const torch::Tensor& k_cache) {
+  PAD_ASSERT(slots.is_cuda() && slots.dim() == 1 && is_index(slots), "slots must be a 1-D int32 or int64 GPU tensor");
+  TORCH_CHECK(slots.device() == k_cache.device(), "pa_decode: all tensors must be on the same device");
+  return slots.contiguous();
+}
+
+void check_index(const torch::Tensor& block_table, const torch::Tensor& seq_lens, const torch::Tensor& k_cache) {
+  PAD_ASSERT(block_table.is_cuda() && seq_lens.is_cuda(), "block_table and seq_lens must be GPU tensors");
+  PAD_ASSERT(block_table.dim() == 2 && seq_lens.dim() == 1 && seq_lens.size(0) == block_table.size(0),
+             "block_table must be [batch, max_pages] and seq_lens [batch]");
+  PAD_ASSERT(is_index(block_table) && is_index(seq_lens), "block_table and seq_lens must be int32 or int64");
+  PAD_ASSERT(block_table.size(1) <= INT32_MAX && seq_lens.size(0) <= INT32_MAX, "block_table too large");
+  TORCH_CHECK(block_table.device() == k_cache.device() && seq_lens.device() == k_cache.device(),
               "pa_decode: all tensors must be on the same device");
+}
+
+// 16-byte rows, as the kernels need them; copied if they are not.
+torch::Tensor aligned_rows(const torch::Tensor& x) {
+  const bool ok = x.stride(2) == 1 && x.stride(1) % 8 == 0 && x.stride(0) % 8 == 0 &&
+                  reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  return ok ? x : x.contiguous().data_ptr() == x.data_ptr() ? x.clone(at::MemoryFormat::Contiguous) : x.contiguous();
+}
+
+pad_kv_rows rows_desc(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& slots) {
   pad_kv_rows r;
   std::memset(&r, 0, sizeof(r));
   r.k = k.data_ptr();
@@ -665,25 +750,46 @@ hipStream_t current_stream(const torch::Tensor& t) {
   return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device()).stream();
 }
 
+bool rows_fit(const pad_kv_cache& c, at::ScalarType rows) {
+  return (c.kv_format != PAD_KV_FP16 || rows == at::kHalf) && (c.kv_format != PAD_KV_BF16 || rows == at::kBFloat16);
+}
+
 void kv_append(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor slots,
-               OptTensor k_scales, OptTensor v_scales, double k_scale, double v_scale, OptTensor weights,
-               OptTensor positions, OptTensor token_weights, OptTensor token_positions) {
-  const pad_kv_cache c =
-      cache_desc(k_cache, v_cache, k_scales, v_scales, weights, positions, k_scale, v_scale, k.size(2));
-  const pad_kv_rows r = rows_desc(k, v, slots);
-  check_same_gpu(k_cache, {&token_weights, &token_positions});
-  TORCH_CHECK(k.device() == k_cache.device(), "pa_decode: all tensors must be on the same device");
-  TORCH_CHECK(k.size(1) == k_cache.size(2), "pa_decode: k and v do not match the caches' heads");
-  TORCH_CHECK(!token_weights.has_value() ||
-                  (token_weights->scalar_type() == at::kFloat && token_weights->is_contiguous() &&
-                   token_weights->numel() == k.size(0) * k.size(1)),
-              "pa_decode: token_weights must be contiguous float32 [tokens, num_kv_heads]");
-  TORCH_CHECK(!token_positions.has_value() ||
-                  (token_positions->scalar_type() == at::kInt && token_positions->is_contiguous() &&
-                   token_positions->numel() == k.size(0)),
-              "pa_decode: token_positions must be contiguous int32 [tokens]");
+               py::object k_scale, py::object v_scale, OptTensor weights, OptTensor positions, OptTensor token_weights,
+               OptTensor token_positions) {
+  pad_kv_cache c = cache_desc(k_cache, v_cache, k_scale, v_scale);
+  check_written(k_cache, v_cache, k_scale, v_scale);
+  PAD_ASSERT(k.is_cuda() && v.is_cuda(), "k and v must be GPU tensors");
+  PAD_ASSERT(is_row_type(k) && v.scalar_type() == k.scalar_type(), "k and v must both be float16 or both bfloat16");
+  PAD_ASSERT(k.dim() == 3 && v.sizes() == k.sizes() && k.size(1) == c.num_kv_heads && k.size(2) == c.head_dim,
+             "k and v must be [tokens, num_kv_heads, head_dim] of the caches");
+  PAD_ASSERT(rows_fit(c, k.scalar_type()), "16-bit caches take rows of their own type");
+  TORCH_CHECK(k.device() == k_cache.device() && v.device() == k_cache.device(),
+              "pa_decode: all tensors must be on the same device");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+  slots = check_slots(slots, k_cache);
+  PAD_ASSERT(slots.size(0) == k.size(0), "slots must name one slot per row");
+  add_state(&c, k_cache, weights, positions);
+  PAD_ASSERT(positions.has_value() == token_positions.has_value(), "positions and token_positions go together");
+  PAD_ASSERT(weights.has_value() || !token_weights.has_value(), "token_weights need weights");
+  if (token_weights.has_value()) {
+    PAD_ASSERT(token_weights->is_cuda() && token_weights->scalar_type() == at::kFloat && token_weights->dim() == 2 &&
+                   token_weights->size(0) == k.size(0) && token_weights->size(1) == k.size(1),
+               "token_weights must be float32 [tokens, num_kv_heads] on the GPU");
+    TORCH_CHECK(token_weights->device() == k_cache.device(), "pa_decode: all tensors must be on the same device");
+    token_weights = token_weights->contiguous();
+  }
+  if (token_positions.has_value()) {
+    PAD_ASSERT(token_positions->is_cuda() && is_index(*token_positions) && token_positions->dim() == 1 &&
+                   token_positions->size(0) == k.size(0),
+               "token_positions must be int32 or int64 [tokens] on the GPU");
+    TORCH_CHECK(token_positions->device() == k_cache.device(), "pa_decode: all tensors must be on the same device");
+    token_positions = as_int32(*token_positions).contiguous();
+  }
   if (k.size(0) == 0) return;
-  c10::hip::HIPGuardMasqueradingAsCUDA guard(k.device());
+  k = aligned_rows(k);
+  v = aligned_rows(v);
+  const pad_kv_rows r = rows_desc(k, v, slots);
   const int st = pad_kv_append(&c, &r, token_weights.has_value() ? token_weights->data_ptr<float>() : nullptr,
                                token_positions.has_value() ? token_positions->data_ptr<int32_t>() : nullptr,
                                current_stream(k));
@@ -691,17 +797,22 @@ void kv_append(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::T
 }
 
 std::tuple<torch::Tensor, torch::Tensor> kv_read(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor slots,
-                                                 OptTensor k_scales, OptTensor v_scales, double k_scale,
-                                                 double v_scale, int64_t head_dim, bool bf16) {
-  const pad_kv_cache c = cache_desc(k_cache, v_cache, k_scales, v_scales, c10::nullopt, c10::nullopt, k_scale, v_scale,
-                                    head_dim);
-  TORCH_CHECK(slots.is_cuda() && slots.dim() == 1, "pa_decode: slots must be a 1-D GPU tensor");
+                                                 py::object k_scale, py::object v_scale, py::object dtype) {
+  const pad_kv_cache c = cache_desc(k_cache, v_cache, k_scale, v_scale);
+  at::ScalarType type = c.kv_format == PAD_KV_BF16 ? at::kBFloat16 : at::kHalf;
+  if (!dtype.is_none()) {
+    PAD_ASSERT(THPDtype_Check(dtype.ptr()), "dtype must be float16 or bfloat16");
+    type = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
+  }
+  PAD_ASSERT(type == at::kHalf || type == at::kBFloat16, "dtype must be float16 or bfloat16");
+  PAD_ASSERT(rows_fit(c, type), "16-bit caches are read in their own type");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
-  const auto options = k_cache.options().dtype(bf16 ? at::kBFloat16 : at::kHalf);
-  auto k = torch::empty({slots.size(0), k_cache.size(2), head_dim}, options);
-  auto v = torch::empty_like(k);
-  const pad_kv_rows r = rows_desc(k, v, slots);
+  slots = check_slots(slots, k_cache);
+  const auto options = k_cache.options().dtype(type);
+  auto k = torch::empty({slots.size(0), c.num_kv_heads, c.head_dim}, options);
+  auto v = torch::empty({slots.size(0), c.num_kv_heads, c.head_dim}, options);
   if (slots.size(0) > 0) {
+    const pad_kv_rows r = rows_desc(k, v, slots);
     const int st = pad_kv_read(&c, &r, current_stream(k));
     TORCH_CHECK(st == PAD_OK, "pa_decode: ", pad_status_string(st));
   }
@@ -709,31 +820,39 @@ std::tuple<torch::Tensor, torch::Tensor> kv_read(torch::Tensor k_cache, torch::T
 }
 
 torch::Tensor kv_evict(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor weights, torch::Tensor positions,
-                       torch::Tensor block_table, torch::Tensor seq_lens, OptTensor k_scales, OptTensor v_scales,
-                       OptTensor keeps, int64_t keep, int64_t recent, int64_t head_dim) {
-  const pad_kv_cache c = cache_desc(k_cache, v_cache, k_scales, v_scales, weights, positions, 1.0, 1.0, head_dim);
-  const OptTensor bt = block_table, sl = seq_lens;
-  check_same_gpu(k_cache, {&bt, &sl, &keeps});
-  TORCH_CHECK(block_table.scalar_type() == at::kInt && seq_lens.scalar_type() == at::kInt && block_table.dim() == 2 &&
-                  seq_lens.dim() == 1 && block_table.size(0) == seq_lens.size(0),
-              "pa_decode: block_table [batch, max_pages] and seq_lens [batch] must be int32");
-  TORCH_CHECK(!keeps.has_value() || (keeps->scalar_type() == at::kInt && keeps->is_contiguous() &&
-                                     keeps->numel() == seq_lens.size(0)),
-              "pa_decode: keep must be contiguous int32 [batch]");
-  TORCH_CHECK(block_table.size(1) <= INT32_MAX && seq_lens.size(0) <= INT32_MAX && keep >= 0 && keep <= INT32_MAX &&
-                  recent >= 0 && recent <= INT32_MAX,
-              "pa_decode: keep or recent out of range");
+                       torch::Tensor block_table, torch::Tensor seq_lens, py::object keep, int64_t recent,
+                       py::object k_scale, py::object v_scale) {
+  // An eviction moves bytes: fp8 caches need no scales.
+  pad_kv_cache c = cache_desc(k_cache, v_cache, k_scale, v_scale);
+  check_written(k_cache, v_cache, k_scale, v_scale);
+  add_state(&c, k_cache, weights, positions);
+  check_index(block_table, seq_lens, k_cache);
+  PAD_ASSERT(recent >= 0 && recent <= INT32_MAX, "recent must be at least 0");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+  block_table = as_int32(block_table);
+  seq_lens = as_int32(seq_lens);
+  pad_kv_evict_call e;
+  std::memset(&e, 0, sizeof(e));
+  torch::Tensor keeps;
+  if (THPVariable_Check(keep.ptr())) {
+    keeps = THPVariable_Unpack(keep.ptr());
+    PAD_ASSERT(keeps.is_cuda() && is_index(keeps) && keeps.dim() == 1 && keeps.size(0) == seq_lens.size(0),
+               "keep must be an int, or int32 [batch] on the GPU");
+    TORCH_CHECK(keeps.device() == k_cache.device(), "pa_decode: all tensors must be on the same device");
+    keeps = as_int32(keeps).contiguous();
+    e.keeps = keeps.data_ptr<int32_t>();
+  } else {
+    const int64_t n = py::cast<int64_t>(keep);
+    PAD_ASSERT(n >= 1 && n <= INT32_MAX, "keep must be at least 1");
+    e.keep = static_cast<int32_t>(n);
+  }
   auto new_lens = torch::empty({seq_lens.size(0)}, seq_lens.options());
   size_t bytes = 0;
   int st = pad_kv_evict_workspace_bytes(seq_lens.size(0), c.num_kv_heads, block_table.size(1), c.page_size, &bytes);
   TORCH_CHECK(st == PAD_OK, "pa_decode: ", pad_status_string(st));
   auto ws = torch::empty({static_cast<int64_t>(bytes)}, k_cache.options().dtype(at::kByte));
-  pad_kv_evict_call e;
-  std::memset(&e, 0, sizeof(e));
   e.block_table = block_table.data_ptr<int32_t>();
   e.seq_lens = seq_lens.data_ptr<int32_t>();
-  e.keeps = keeps.has_value() ? keeps->data_ptr<int32_t>() : nullptr;
   e.new_lens = new_lens.data_ptr<int32_t>();
   e.workspace = ws.data_ptr();
   e.workspace_bytes = bytes;
@@ -742,7 +861,6 @@ torch::Tensor kv_evict(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tens
   e.sl_stride = seq_lens.stride(0);
   e.batch = static_cast<int32_t>(seq_lens.size(0));
   e.max_pages = static_cast<int32_t>(block_table.size(1));
-  e.keep = static_cast<int32_t>(keep);
   e.recent = static_cast<int32_t>(recent);
   st = pad_kv_evict(&c, &e, current_stream(k_cache));
   TORCH_CHECK(st == PAD_OK, "pa_decode: ", pad_status_string(st));
@@ -752,28 +870,34 @@ torch::Tensor kv_evict(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tens
 // Decode over MX4 caches, or with accumulated weights, or both: forward()'s plan,
 // scratch and stream; the scores' scratch comes from PyTorch's allocator.
 torch::Tensor cache_decode(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor block_table,
-                           torch::Tensor seq_lens, OptTensor k_scales, OptTensor v_scales, OptTensor weights,
-                           double scale, double k_scale, double v_scale, int64_t num_splits) {
-  TORCH_CHECK(q.dim() == 3, "pa_decode: q must be [batch, num_q_heads, head_dim]");
-  const pad_kv_cache desc =
-      cache_desc(k_cache, v_cache, k_scales, v_scales, weights, c10::nullopt, k_scale, v_scale, q.size(2));
+                           torch::Tensor seq_lens, py::object k_scale, py::object v_scale, OptTensor weights,
+                           c10::optional<double> scale, c10::optional<int64_t> num_splits) {
+  PAD_ASSERT(q.is_cuda() && is_row_type(q) && q.dim() == 3,
+             "q must be a float16 or bfloat16 GPU tensor [batch, num_q_heads, head_dim]");
+  pad_kv_cache desc = cache_desc(k_cache, v_cache, k_scale, v_scale);
   const bool mx4 = desc.kv_format == PAD_KV_MX4;
-  TORCH_CHECK(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16,
-              "pa_decode: q must be float16 or bfloat16");
-  const OptTensor oq = q, bt = block_table, sl = seq_lens;
-  check_same_gpu(k_cache, {&oq, &bt, &sl});
-  TORCH_CHECK(block_table.scalar_type() == at::kInt && seq_lens.scalar_type() == at::kInt && block_table.dim() == 2 &&
-                  seq_lens.dim() == 1 && block_table.size(0) == q.size(0) && seq_lens.size(0) == q.size(0),
-              "pa_decode: block_table [batch, max_pages] and seq_lens [batch] must be int32");
-  TORCH_CHECK(num_splits >= 0 && num_splits <= INT32_MAX, "pa_decode: num_splits out of range");
+  PAD_ASSERT(mx4 || weights.has_value(), "MX4 caches are uint8 (or float4_e2m1fn_x2) codes");
+  PAD_ASSERT(rows_fit(desc, q.scalar_type()), "16-bit caches must have q's type");
+  PAD_ASSERT(q.size(2) == desc.head_dim, "q head_dim must match the KV cache head_dim");
+  PAD_ASSERT(q.size(1) > 0 && q.size(1) % desc.num_kv_heads == 0, "num_q_heads must be divisible by num_kv_heads (GQA)");
+  PAD_ASSERT(q.size(1) / desc.num_kv_heads <= PAD_MAX_GQA, "GQA group larger than 16");
+  add_state(&desc, k_cache, weights, c10::nullopt);
+  check_index(block_table, seq_lens, k_cache);
+  PAD_ASSERT(block_table.size(0) == q.size(0), "block_table must be [batch, max_pages]");
+  PAD_ASSERT(!num_splits.has_value() || (*num_splits >= 1 && *num_splits <= INT32_MAX), "num_splits must be >= 1");
+  TORCH_CHECK(q.device() == k_cache.device(), "pa_decode: all tensors must be on the same device");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  block_table = as_int32(block_table);
+  seq_lens = as_int32(seq_lens);
   auto out = torch::empty({q.size(0), q.size(1), q.size(2)}, q.options());
   if (q.size(0) == 0) return out;
+  q = aligned_rows(q);
+  const int splits = num_splits.has_value() ? static_cast<int>(*num_splits) : 0;
   pad_decode_dims d;
   fill_dims(q, k_cache, v_cache, block_table, seq_lens, out, &d);
   pad_decode_plan_t plan;
   const int cus = cached_cus(q.get_device());
-  int st = pad_decode_plan(&d, static_cast<int>(num_splits), cus, &plan);
+  int st = pad_decode_plan(&d, splits, cus, &plan);
   TORCH_CHECK(st == PAD_OK, "pa_decode: ", pad_status_string(st));
   hipStream_t stream = current_stream(q);
   pad_cache_call cc;
@@ -785,16 +909,18 @@ torch::Tensor cache_decode(torch::Tensor q, torch::Tensor k_cache, torch::Tensor
   c.block_table = block_table.data_ptr<int32_t>();
   c.seq_lens = seq_lens.data_ptr<int32_t>();
   c.out = out.data_ptr();
-  const LaunchScratch scratch = launch_scratch(q, stream, d, static_cast<int>(num_splits), cus, false, plan);
+  const LaunchScratch scratch = launch_scratch(q, stream, d, splits, cus, false, plan);
   c.workspace = scratch.workspace;
   c.workspace_bytes = scratch.workspace_bytes;
   c.counters = scratch.counters;
   c.num_counters = scratch.num_counters;
-  c.scale = static_cast<float>(scale);
-  c.num_splits = static_cast<int32_t>(num_splits);
-  c.kv_format = mx4 ? (q.scalar_type() == at::kHalf ? PAD_KV_MX4 : PAD_KV_MX4_BF16) : cache_format(q, k_cache, v_cache);
-  c.k_scale = static_cast<float>(k_scale);
-  c.v_scale = static_cast<float>(v_scale);
+  c.scale = scale.has_value() ? static_cast<float>(*scale)
+                              : static_cast<float>(1.0 / std::sqrt(static_cast<double>(desc.head_dim)));
+  c.num_splits = splits;
+  const bool bf16 = q.scalar_type() == at::kBFloat16;
+  c.kv_format = mx4 ? (bf16 ? PAD_KV_MX4_BF16 : PAD_KV_MX4) : cache_format(q, k_cache, v_cache);
+  c.k_scale = desc.k_scale;
+  c.v_scale = desc.v_scale;
   cc.k_scales = desc.k_scales;
   cc.v_scales = desc.v_scales;
   std::memcpy(cc.ks_stride, desc.ks_stride, sizeof(cc.ks_stride));
