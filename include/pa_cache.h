@@ -41,14 +41,16 @@ extern "C" {
  *   call: as for pad_decode_launch_call(), with the dense page index, no work
  *     list, engine 0, and kv_format one of pa_decode.h's or the two above.  Over
  *     MX4 caches k_cache and v_cache are the codes and dims' k_stride and
- *     v_stride count bytes (rows 16-byte aligned, 8 at head_dim 64); k_scale and
+ *     v_stride count bytes (rows 16-byte aligned, 8 at head_dim 64; page and slot
+ *     strides below 2^32, as the scales'); k_scale and
  *     v_scale are not read.
  *   k_scales, v_scales, ks_stride, vs_stride: MX4 scale bytes; strides of page,
  *     slot and kv head.
  *   weights, w_stride: NULL, or where the softmax weights of every token, summed
  *     over the query heads of its kv head, are added (strides in elements).
  *   logits, logits_bytes: scratch of pad_cache_logits_bytes(), with weights.
- * Scratch (workspace, counters) as for pad_decode_launch(). */
+ * Scratch (workspace, counters): pad_cache_scratch(); with less than that a call
+ * may run another kernel, or return PAD_ERR_WORKSPACE. */
 typedef struct pad_cache_call {
   pad_decode_call call;
   const uint8_t* k_scales;
@@ -60,6 +62,13 @@ typedef struct pad_cache_call {
   void* logits;
   size_t logits_bytes;
 } pad_cache_call;
+
+/* Workspace bytes and counters (zeroed once, left at zero) of a
+ * pad_cache_decode() over caches of kv_format; num_cus <= 0 means 256.  Host
+ * only. */
+int pad_cache_scratch(const pad_decode_dims* dims, int kv_format,
+                      int num_splits, int num_cus, size_t* bytes,
+                      int64_t* count);
 
 /* Bytes of the scores of one decode: 4 per (query head, token of a table row),
  * and 4 per (sequence, query head).  Host only. */

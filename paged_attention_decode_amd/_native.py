@@ -238,6 +238,9 @@ class PadKvEvictCall(ctypes.Structure):
 
 # include/pa_cache.h
 CACHE_SIGNATURES = {
+    "pad_cache_scratch": (
+        [ctypes.POINTER(PadDims), ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_size_t),
+         ctypes.POINTER(ctypes.c_int64)], ctypes.c_int),
     "pad_cache_logits_bytes": ([ctypes.POINTER(PadDims), ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
     "pad_cache_decode": ([ctypes.POINTER(PadCacheCall), ctypes.POINTER(PadDims), _VP], ctypes.c_int),
     "pad_kv_append": ([ctypes.POINTER(PadKvCache), ctypes.POINTER(PadKvRows), _VP, _VP, _VP], ctypes.c_int),

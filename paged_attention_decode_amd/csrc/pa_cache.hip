@@ -269,14 +269,14 @@ hipError_t launch_accumulate(const Phase1Args& p, float* weights, const int64_t*
   a.swh = w_stride[2];
   a.num_pages = p.num_pages;
   a.gqa = p.gqa;
-  a.hkv = p.hkv;
+  a.hkv = p.hq / p.gqa;  // (a range launch's hkv counts head groups)
   a.ps = p.ps;
   a.ps_shift = p.ps_shift;
   a.max_pages = p.max_pages;
-  const int64_t units = (int64_t)p.batch * p.hkv;
+  const int64_t units = (int64_t)p.batch * a.hkv;
   const int64_t chunks = ((int64_t)p.max_pages * p.ps + 255) / 256;
   const int64_t most = 4096 / units > 1 ? 4096 / units : 1;
-  hipLaunchKernelGGL(pad_accumulate_kernel, dim3((unsigned)(chunks < most ? chunks : most), p.hkv, p.batch), dim3(256),
+  hipLaunchKernelGGL(pad_accumulate_kernel, dim3((unsigned)(chunks < most ? chunks : most), a.hkv, p.batch), dim3(256),
                      0, st, a);
   return hipGetLastError();
 }

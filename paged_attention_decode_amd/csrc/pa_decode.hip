@@ -445,7 +445,7 @@ constexpr int64_t kRangeCallBytes = 1 << 27;
 // calls with few units keep the per-unit kernel's shorter merge (32/8 heads,
 // 4 x 8192: 26.3 against 28.6-32 us).
 static RangeShape range_shape(const pad_decode_dims* d, int num_splits, int num_cus, int engine, bool csr,
-                              int kv_bytes) {
+                              int kv_bytes, bool mx4 = false) {
   RangeShape r = {0, 0, 0, 0, 0, 0, 0};
 #ifdef PAD_TIMELINE
   return r;  // the phase stamps are the per-unit kernel's
@@ -470,7 +470,7 @@ static RangeShape range_shape(const pad_decode_dims* d, int num_splits, int num_
   // [1, 4608] of 24/6 1.05), and so does head_dim 64 (9 x [1, 7264] 1.32).
   if (units * 4 <= num_cus || units * 2 == num_cus || latency_bound_shape(d, num_cus, csr)) return r;
   if (r.nh_shift == 2 && (r.nw == kMaxWaves / 2 ? units * 2 < num_cus : kv_bytes == 1 && units * 3 <= num_cus)) return r;
-  const int64_t page_bytes = ((int64_t)d->page_size * d->head_dim * kv_bytes * 2) << r.nh_shift;
+  const int64_t page_bytes = ((int64_t)d->page_size * d->head_dim * (mx4 ? 1 : kv_bytes * 2)) << r.nh_shift;
   const int64_t row_bytes = plan_pages_per_seq(d, csr) * (((int64_t)d->page_size * d->head_dim * 4) << r.nh_shift);
   if (row_bytes < kRangeRowBytes || (units >> r.nh_shift) * row_bytes < kRangeCallBytes) return r;
   // Positions are counted in 32 bits (twice the pages at most, and unit_extra).
@@ -614,13 +614,13 @@ static size_t worklist_bytes_for(const pad_decode_plan_t& plan, const pad_decode
 // CSR: bt = indices, indptr / lpl given, sl unused (dims->max_pages is the
 // number of entries in indices).  io: also check q/k/v/out and the scratch
 // (a work-list plan reads only the index arrays).  list_bytes: size of the
-// work list the launch reads or the plan writes, if there is one.  per_unit:
-// the per-unit kernel, whatever the shape.
+// work list the launch reads or the plan writes, if there is one.  mx4: MX4
+// caches (kv_bytes 1).
 static int setup_launch(const void* q, const void* k, const void* v, const int32_t* bt, const int32_t* sl,
                         const int32_t* indptr, const int32_t* lpl, void* out, void* ws, size_t ws_bytes,
                         int32_t* counters, int64_t num_counters, const pad_decode_dims* d, float scale,
                         int num_splits, int engine, bool io, Launch* L, int kv_bytes = 2,
-                        size_t list_bytes = SIZE_MAX, bool per_unit = false) {
+                        size_t list_bytes = SIZE_MAX, bool mx4 = false) {
   if (engine != 0 && engine != 1) return PAD_ERR_INVALID_SHAPE;
   // Page ids are bounds-checked against num_pages on the device (an id
   // outside [0, num_pages) reads page 0), so a launch that reads pages needs
@@ -634,8 +634,7 @@ static int setup_launch(const void* q, const void* k, const void* v, const int32
   int pps_full = 0;
   st = plan_units(d, num_splits, cus, engine, csr, &plan, kv_bytes, &pps_full);
   if (st != PAD_OK) return st;
-  RangeShape rs = range_shape(d, num_splits, cus, engine, csr, kv_bytes);
-  if (per_unit) rs.groups = 0;
+  const RangeShape rs = range_shape(d, num_splits, cus, engine, csr, kv_bytes, mx4);
   // The range kernel runs where its scratch and its list fit (an fp8 launch's
   // own grid may have fewer workgroups than the range launch, and a list of
   // that size stays good for it).
@@ -736,6 +735,7 @@ static int setup_launch(const void* q, const void* k, const void* v, const int32
   a.sksp = a.skss = a.sksh = a.svsp = a.svss = a.svsh = 0;
   a.logits = a.lse = nullptr;
   a.slog = 0;
+  a.hq = d->num_q_heads;
   a.fold_polls = 0;
   // The shared fold waits for a unit's other workgroups: only where the whole
   // grid can run at once, each unit has group counters, and a unit can get
@@ -886,6 +886,10 @@ static int launch_cache_call(const pad_cache_call* cc, const pad_decode_dims* d,
     if (c.engine != 0) return PAD_ERR_KV_FORMAT;
     if (d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256) return PAD_ERR_UNSUPPORTED_HEAD_DIM;
     if (d->batch > 0 && (!cc->k_scales || !cc->v_scales)) return PAD_ERR_NULL_POINTER;
+    // Strides are multiplied as unsigned 32-bit values.
+    for (int i = 0; i < 2; ++i)
+      for (int64_t x : {d->k_stride[i], d->v_stride[i], cc->ks_stride[i], cc->vs_stride[i]})
+        if (x < 0 || x > UINT32_MAX) return PAD_ERR_STRIDE;
     // A lane reads 16 bytes of a row at once, 8 at head_dim 64.
     if (d->head_dim >= 128 && ((d->k_stride[0] | d->k_stride[1] | d->k_stride[2] | d->v_stride[0] | d->v_stride[1] |
                                 d->v_stride[2]) & 15))
@@ -894,13 +898,16 @@ static int launch_cache_call(const pad_cache_call* cc, const pad_decode_dims* d,
     st = check_kv_format(c.kv_format, c.engine, d, c.k_scale, c.v_scale);
     if (st != PAD_OK) return st;
     if (c.engine != 0) return PAD_ERR_KV_FORMAT;
+    // A block's rows are addressed with 32-bit offsets.
+    for (int64_t x : {d->k_stride[1], d->v_stride[1]})
+      if (x < 0 || x > UINT32_MAX / 32 - 64) return PAD_ERR_STRIDE;
   }
   // The launch counts the tokens of a table row in 32 bits.
   if ((int64_t)d->max_pages * d->page_size > INT32_MAX - 4096) return PAD_ERR_INVALID_SHAPE;
   Launch L;
   st = setup_launch(c.q, c.k_cache, c.v_cache, c.block_table, c.seq_lens, nullptr, nullptr, c.out, c.workspace,
                     c.workspace_bytes, c.counters, c.num_counters, d, c.scale, c.num_splits, 0, true, &L,
-                    mx4 || fp8 ? 1 : 2, SIZE_MAX, true);
+                    mx4 || fp8 ? 1 : 2, SIZE_MAX, mx4);
   if (st != PAD_OK || L.empty) return st;
   if (fp8) {
     L.a.scale_log2 *= c.k_scale;
@@ -924,11 +931,11 @@ static int launch_cache_call(const pad_cache_call* cc, const pad_decode_dims* d,
   }
   hipError_t e;
   if (mx4)
-    e = launch_mx4(L.a, d->head_dim, kvf | (cc->weights ? kKvWeights : 0), L.grid, L.nw, L.lds, hs);
+    e = launch_mx4(L.a, L.range, d->head_dim, kvf | (cc->weights ? kKvWeights : 0), L.grid, L.nw, L.lds, hs);
   else if (fp8)
-    e = launch_weights_fp8(L.a, d->head_dim, kvf, L.grid, L.nw, L.lds, hs);
+    e = launch_weights_fp8(L.a, L.range, d->head_dim, kvf, L.grid, L.nw, L.lds, hs);
   else
-    e = launch_weights(L.a, d->head_dim, kvf, L.grid, L.nw, L.lds, hs);
+    e = launch_weights(L.a, L.range, d->head_dim, kvf, L.grid, L.nw, L.lds, hs);
   if (e != hipSuccess) return PAD_ERR_LAUNCH;
   if (cc->weights && d->max_pages > 0 && launch_accumulate(L.a, cc->weights, cc->w_stride, hs) != hipSuccess)
     return PAD_ERR_LAUNCH;
@@ -1254,6 +1261,21 @@ int pad_cache_logits_bytes(const pad_decode_dims* dims, size_t* bytes) {
   if (st != PAD_OK) return st;
   if (!bytes) return PAD_ERR_NULL_POINTER;
   *bytes = pad::logits_bytes_of(dims);
+  return PAD_OK;
+}
+
+int pad_cache_scratch(const pad_decode_dims* dims, int kv_format, int num_splits, int num_cus, size_t* bytes,
+                      int64_t* count) {
+  if (!bytes || !count) return PAD_ERR_NULL_POINTER;
+  const bool mx4 = kv_format == PAD_KV_MX4 || kv_format == PAD_KV_MX4_BF16;
+  if (!mx4 && pad::check_kv_format(kv_format, 0, dims, 1.0f, 1.0f) != PAD_OK) return PAD_ERR_KV_FORMAT;
+  const int kv_bytes = mx4 || pad::kv_format_fp8(kv_format) ? 1 : 2;
+  pad_decode_plan_t p;
+  const int st = pad::plan_units(dims, num_splits, num_cus, 0, false, &p, kv_bytes);
+  if (st != PAD_OK) return st;
+  const pad::RangeShape r = pad::range_shape(dims, num_splits, num_cus, 0, false, kv_bytes, mx4);
+  *bytes = r.groups > 0 && r.workspace_bytes > p.workspace_bytes ? r.workspace_bytes : p.workspace_bytes;
+  *count = r.groups > 0 && r.counters > p.counters ? r.counters : p.counters;
   return PAD_OK;
 }
 

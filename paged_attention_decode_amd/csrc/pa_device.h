@@ -98,6 +98,7 @@ struct Phase1Args {
   float* logits;
   float* lse;
   int64_t slog;
+  int hq;          // query heads
 #ifdef PAD_TIMELINE
   int tl_launch;   // ring slot of this launch's stamps
 #endif
@@ -501,6 +502,29 @@ __device__ __forceinline__ void fp8x4_to_16x4(uint32_t w, uint32_t& lo, uint32_t
 // barrier is needed (the waves write identical values).
 template <int D>
 constexpr bool q_in_lds() { return D >= 256; }
+
+// Scores of kKvWeights calls: those of row `row` of kv head kvh, by token.
+__device__ __forceinline__ float* logits_of(const Phase1Args& a, int b, int kvh, int row) {
+  return a.logits + ((int64_t)b * a.hq + kvh * a.gqa + row) * a.slog;
+}
+
+// The first n of four consecutive scores (rows start at any token, so the
+// vector store is aligned to a float only).
+__device__ __forceinline__ void store_logits(float* p, const float (&x)[4], int n) {
+  typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
+  if (n >= 4) {
+    *reinterpret_cast<f4u_t*>(p) = f4u_t{x[0], x[1], x[2], x[3]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i < n) p[i] = x[i];
+  }
+}
+
+// log2 of a query head's normaliser: m in base-2 units, l the sum of 2^(score - m).
+__device__ __forceinline__ void store_lse(const Phase1Args& a, int b, int head, float m, float l) {
+  a.lse[(int64_t)b * a.hq + head] = m + __builtin_amdgcn_logf(l);
+}
 
 // Wave-wide integer reductions: DPP within each 16-lane row, then the four
 // row results combined through readlane (wave-uniform result).

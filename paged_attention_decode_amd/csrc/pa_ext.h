@@ -1,20 +1,22 @@
-// pa_ext.h - launchers of the per-unit kernel's other instantiations, used by
-// the launch path in pa_decode.hip.
+// pa_ext.h - launchers of the decode kernels' other instantiations, used by the
+// launch path in pa_decode.hip.
 #ifndef PA_EXT_H_
 #define PA_EXT_H_
 
-#include "pa_device.h"
+#include "pa_range.h"
 
 namespace pad {
 
 // Decode over MX4 caches (head_dim 64, 128 or 256); kvf: kKvMx4 or kKvMx4B,
-// plus kKvWeights.
-hipError_t launch_mx4(const Phase1Args& a, int head_dim, int kvf, dim3 grid, int nw, size_t lds, hipStream_t st);
+// plus kKvWeights.  range: the range kernel (grid unused), else the per-unit one.
+hipError_t launch_mx4(const RangeArgs& a, bool range, int head_dim, int kvf, dim3 grid, int nw, size_t lds,
+                      hipStream_t st);
 
 // Decode that also writes its scores and normalisers; kvf: a 16-bit
 // (pa_weights.hip) or fp8 (pa_weights_fp8.hip) format, without kKvWeights.
-hipError_t launch_weights(const Phase1Args& a, int head_dim, int kvf, dim3 grid, int nw, size_t lds, hipStream_t st);
-hipError_t launch_weights_fp8(const Phase1Args& a, int head_dim, int kvf, dim3 grid, int nw, size_t lds,
+hipError_t launch_weights(const RangeArgs& a, bool range, int head_dim, int kvf, dim3 grid, int nw, size_t lds,
+                          hipStream_t st);
+hipError_t launch_weights_fp8(const RangeArgs& a, bool range, int head_dim, int kvf, dim3 grid, int nw, size_t lds,
                               hipStream_t st);
 
 // weights += the weights of p's launch (its logits and lse, dense page index).

@@ -24,9 +24,9 @@
 
 namespace pad {
 
-// Waves per SIMD that the kernels are compiled for (registers per lane): the
-// scores' row pointers did not fit 168 registers at head_dim 128.
-constexpr int mx4_waves_per_simd(int d, bool weights) { return d <= 128 ? (d == 128 && weights ? 2 : 3) : 1; }
+// Waves per SIMD that the per-unit kernels are compiled for (registers per lane):
+// head_dim 128 does not fit the 168 of three.
+constexpr int mx4_waves_per_simd(int d) { return d <= 64 ? 3 : d <= 128 ? 2 : 1; }
 
 // One 16x16x32 step on 16-bit operands (8 elements of the contraction a lane).
 template <int KVF>
@@ -60,6 +60,18 @@ __device__ __forceinline__ h8_t mx4x8(uint32_t w, float scale) {
   return __builtin_bit_cast(h8_t, r);
 }
 
+// Two floats rounded to q's type, in a dword.
+template <int KVF>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  if constexpr (q_is_bf16<KVF>()) {
+    typedef float f2_t __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2_t{x, y}, b2_t));
+  } else {
+    return __builtin_bit_cast(uint32_t, h2_t{(_Float16)x, (_Float16)y});
+  }
+}
+
 // A row is NC chunks of up to 32 elements a lane (one scale each), at elements
 // c * 128 + g * kMx4Lane: a load instruction covers whole rows.
 template <int D>
@@ -91,15 +103,16 @@ __device__ __forceinline__ h4_t lds_read_transposed(const char* p) {
   return __builtin_bit_cast(h4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)p));
 }
 
-__device__ __forceinline__ float* logits_of(const Phase1Args& a, int b, int kvh, int row);
-__device__ __forceinline__ void store_logits(float* p, const float (&x)[4], int n);
-
-// MODE: kModeUniform (a 16-token tile lies in one page) or kModeGeneric (each
-// lane finds its own tokens' pages).
+// One wave's part of an item: tokens [t_begin, t_end) (t_begin on a page border,
+// nblk blocks of 16) of kv head kvh, of which the wave takes the pairs of blocks
+// wave, wave + nw, ...; its state goes to place `slot` of sm_ml and sm_o.
+// MODE: kModeUniform (a 16-token block lies in one page) or kModeGeneric (each
+// lane finds its own tokens' pages).  Strides are below 2^32 bytes, and in
+// uniform mode 15 rows apart are below 2^31 (the launcher sees to both).
 template <int D, int MODE, int KVF>
 __device__ __forceinline__ void wave_loop_mx4(const Phase1Args& a, const int32_t* bt_row, int64_t ids_stride, int b,
-                                              int kvh, int t_begin, int t_end, int nblk, int wave, int nw, int lane,
-                                              float2* sm_ml, float* sm_o, char* stage) {
+                                              int kvh, int t_begin, int t_end, int nblk, int wave, int nw, int slot,
+                                              int lane, float2* sm_ml, float* sm_o, char* stage) {
   using Tile = Mx4Tile<D>;
   constexpr int DW = Tile::DW;
   constexpr int NC = Tile::NC;
@@ -121,82 +134,127 @@ __device__ __forceinline__ void wave_loop_mx4(const Phase1Args& a, const int32_t
   };
 
   float m_run = kNegInf;
-  float l_run = 0.f;
   f4_t o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = (f4_t)0.f;
-
-  const char* k_head = reinterpret_cast<const char*>(a.k) + (int64_t)kvh * a.skh;
-  const char* v_head = reinterpret_cast<const char*>(a.v) + (int64_t)kvh * a.svh;
-  const uint8_t* ks_head = a.ks + (int64_t)kvh * a.sksh;
-  const uint8_t* vs_head = a.vs + (int64_t)kvh * a.svsh;
-  const int elem0 = mx4_elem<D>(g, 0);
+  // Row sums of P from one more matrix step with an operand of ones; where the
+  // caller gets the weights, which are unrounded, a lane's own sum.
+  f4_t o_l = (f4_t)0.f;
   float* logit_row = nullptr;
   if constexpr (kv_weights<KVF>()) logit_row = logits_of(a, b, kvh, row_ok ? r16 : 0);
 
-  auto load_row = [&](Tile& t, int u, const char* kp, const char* vp, const uint8_t* ksp, const uint8_t* vsp) {
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const HVec<CW> x = load_hvec_stream<CW>(reinterpret_cast<const _Float16*>(kp + c * 64));
-#pragma unroll
-      for (int w = 0; w < CW; ++w) t.k[u].w[c * CW + w] = x.w[w];
-      t.ks[u][c] = ksp[c * 4];
-    }
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const HVec<CW> x = load_hvec_stream<CW>(reinterpret_cast<const _Float16*>(vp + c * 64));
-#pragma unroll
-      for (int w = 0; w < CW; ++w) t.v[u].w[c * CW + w] = x.w[w];
-      t.vs[u][c] = vsp[c * 4];
-    }
-  };
+  const char* k_head = reinterpret_cast<const char*>(a.k) + (int64_t)kvh * a.skh;
+  const char* v_head = reinterpret_cast<const char*>(a.v) + (int64_t)kvh * a.svh;
+  const char* ks_head = reinterpret_cast<const char*>(a.ks) + (int64_t)kvh * a.sksh;
+  const char* vs_head = reinterpret_cast<const char*>(a.vs) + (int64_t)kvh * a.svsh;
+  const int elem0 = mx4_elem<D>(g, 0);
+  const uint32_t page_limit = (uint32_t)min(a.num_pages, (int64_t)0x7fffffff);
+  auto clamp_id = [&](int id) -> uint32_t { return (uint32_t)id < page_limit ? (uint32_t)id : 0u; };
 
-  // Page ids of the pair the next load() reads: scalar reads (whole-page
-  // tiles), or each lane's own.  They are fetched a pair ahead, before that
-  // pair's predecessor's rows, so that waiting for them waits for no rows.
+  // Where the wave's next pair lies: page (from the item's first) and slot of its
+  // blocks (uniform mode, scalars) or of the lane's tokens; pairs are nw apart.
+  // Page ids are fetched a pair ahead, before its predecessor's rows, so that
+  // waiting for them waits for no rows.  Past the item's end the last page's id
+  // is read again and the tokens are masked.
+  const int lane_row = MODE == kModeUniform ? 0 : r16;
   const int p_first = page_of(a, t_begin);
-  int pid[2], slot[2];
-  auto fetch_ids = [&](int jp) {
+  const int p_last = t_end > t_begin ? page_of(a, t_end - 1) : p_first;
+  const int step_pages = page_of(a, nw * 32);
+  const int step_slots = nw * 32 - step_pages * a.ps;
+  int cur_page[2], cur_slot[2], pid[2], pslot[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int t = wave * 32 + 16 * u + lane_row;
+    cur_page[u] = page_of(a, t);
+    cur_slot[u] = t - cur_page[u] * a.ps;
+  }
+  auto fetch_ids = [&]() {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      if constexpr (MODE == kModeUniform) {
-        const int jb = min(2 * jp + u, nblk - 1);
-        const int page = block_page(a, jb);
-        slot[u] = jb * kBlockTokens - page * a.ps;
-        pid[u] = load_uniform_i32(bt_row + (int64_t)(p_first + page) * ids_stride);
-      } else {
-        const int tk = min(t_begin + jp * 32 + 16 * u + r16, t_end - 1);
-        const int page = page_of(a, tk);
-        slot[u] = tk - page * a.ps;
-        pid[u] = bt_row[(int64_t)page * ids_stride];
+      const int64_t col = (int64_t)min(p_first + cur_page[u], p_last) * ids_stride;
+      if constexpr (MODE == kModeUniform)
+        pid[u] = load_uniform_i32(bt_row + col);
+      else
+        pid[u] = bt_row[col];
+      pslot[u] = cur_slot[u];
+      cur_page[u] += step_pages;
+      cur_slot[u] += step_slots;
+      if (cur_slot[u] >= a.ps) {
+        cur_slot[u] -= a.ps;
+        ++cur_page[u];
       }
     }
   };
-  // Lane offsets inside a tile (whole-page tiles: row r16 of it).
-  const int lane_row = MODE == kModeUniform ? r16 : 0;
-  const int64_t koff = (int64_t)lane_row * a.sks + elem0 / 2;
-  const int64_t voff = (int64_t)lane_row * a.svs + elem0 / 2;
-  const int64_t ksoff = (int64_t)lane_row * a.skss + elem0 / 32;
-  const int64_t vsoff = (int64_t)lane_row * a.svss + elem0 / 32;
-  const int npair = (nblk + 1) >> 1;
-  auto load = [&](Tile& t, int jp) {
-    int64_t page[2], at[2];
+
+  // Rows and scales of one block: from a scalar base with 32-bit lane offsets
+  // (uniform mode), or from each lane's own address.
+  uint32_t koff = (uint32_t)(elem0 / 2), voff = koff, ksoff = (uint32_t)(elem0 / 32), vsoff = ksoff;
+  if constexpr (MODE == kModeUniform) {
+    koff += (uint32_t)r16 * (uint32_t)a.sks;
+    voff += (uint32_t)r16 * (uint32_t)a.svs;
+    ksoff += (uint32_t)r16 * (uint32_t)a.skss;
+    vsoff += (uint32_t)r16 * (uint32_t)a.svss;
+  }
+  constexpr int kStream = 2;  // NT
+  auto load_codes = [&](HVec<DW>& x, const char* base, uint32_t off) {
+    if constexpr (MODE == kModeUniform) {
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(base, 0xffffffffu);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if constexpr (CW == 4) {
+          const u4_t w = __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(r, off + c * 64, 0, kStream));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x.w[c * 4 + j] = w[j];
+        } else {
+          const u2_t w = __builtin_bit_cast(u2_t, __builtin_amdgcn_raw_buffer_load_b64(r, off + c * 64, 0, kStream));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) x.w[c * 2 + j] = w[j];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const HVec<CW> w = load_hvec_stream<CW>(reinterpret_cast<const _Float16*>(base + off + c * 64));
+#pragma unroll
+        for (int j = 0; j < CW; ++j) x.w[c * CW + j] = w.w[j];
+      }
+    }
+  };
+  auto load_scales = [&](uint32_t (&x)[NC], const char* base, uint32_t off) {
+    if constexpr (MODE == kModeUniform) {
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(base, 0xffffffffu);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) x[c] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, off + c * 4, 0, 0);
+    } else {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) x[c] = (uint8_t)base[off + c * 4];
+    }
+  };
+  auto at = [](const char* head, uint32_t page, int64_t page_bytes, uint32_t row, int64_t row_bytes) {
+    return head + (uint64_t)page * (uint32_t)page_bytes + (uint64_t)row * (uint32_t)row_bytes;
+  };
+  auto load = [&](Tile& t) {
+    uint32_t page[2], row[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      page[u] = clamp_page(pid[u], a.num_pages);
-      at[u] = slot[u];
+      page[u] = clamp_id(pid[u]);
+      row[u] = (uint32_t)pslot[u];
     }
-    fetch_ids(min(jp + nw, npair - 1));
+    fetch_ids();
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      load_row(t, u, k_head + page[u] * a.skp + at[u] * a.sks + koff, v_head + page[u] * a.svp + at[u] * a.svs + voff,
-               ks_head + page[u] * a.sksp + at[u] * a.skss + ksoff,
-               vs_head + page[u] * a.svsp + at[u] * a.svss + vsoff);
+    for (int u = 0; u < 2; ++u) {
+      load_codes(t.k[u], at(k_head, page[u], a.skp, row[u], a.sks), koff);
+      load_scales(t.ks[u], at(ks_head, page[u], a.sksp, row[u], a.skss), ksoff);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      load_codes(t.v[u], at(v_head, page[u], a.svp, row[u], a.svs), voff);
+      load_scales(t.vs[u], at(vs_head, page[u], a.svsp, row[u], a.svss), vsoff);
+    }
   };
 
   auto compute = [&](Tile& t, int jp) {
     const int t0 = t_begin + jp * 32;
-    const bool full = t0 + 32 <= t_end;
     float x[2][4];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -207,7 +265,7 @@ __device__ __forceinline__ void wave_loop_mx4(const Phase1Args& a, const int32_t
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[u][i] = sacc[i] * a.scale_log2;
     }
-    if (!full) {
+    if (t0 + 32 > t_end) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
@@ -228,47 +286,34 @@ __device__ __forceinline__ void wave_loop_mx4(const Phase1Args& a, const int32_t
     }
     float bm = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                      fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-    bm = fmaxf(bm, shfl_xor_f(bm, 16));
-    bm = fmaxf(bm, shfl_xor_f(bm, 32));
-    // Lazy rescaling, as in wave_loop_mfma: a pair holds at least one token.
+    // Lazy rescaling, as in the other loops: whether any score exceeds the
+    // reference by the slack needs only each lane's own maximum.  A pair holds
+    // at least one token, so the row's is finite.
     if (__builtin_amdgcn_ballot_w64(bm > m_run + kRescaleSlack) != 0) {
+      bm = fmaxf(bm, shfl_xor_f(bm, 16));
+      bm = fmaxf(bm, shfl_xor_f(bm, 32));
       const float m_new = fmaxf(m_run, bm);
       const float alpha = exp2_fast(m_run - m_new);
-      l_run *= alpha;
+      o_l[0] *= alpha;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
       m_run = m_new;
     }
     // P rounded to q's type; l sums the rounded weights that P.V uses (the
     // unrounded ones where the caller gets the weights).
-    h8_t ph;
-    float psum = 0.f;
-    if constexpr (q_is_bf16<KVF>()) {
-      typedef float f2_t __attribute__((ext_vector_type(2)));
-      typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
-      u4_t w;
+    u4_t pw;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f2_t pf = {exp2_fast(x[j >> 1][2 * (j & 1)] - m_run), exp2_fast(x[j >> 1][2 * (j & 1) + 1] - m_run)};
-        const uint32_t pr = __builtin_bit_cast(uint32_t, __builtin_convertvector(pf, b2_t));
-        w[j] = pr;
-        if constexpr (kv_weights<KVF>())
-          psum += pf.x + pf.y;
-        else
-          psum += __uint_as_float(pr << 16) + __uint_as_float(pr & 0xffff0000u);
-      }
-      ph = __builtin_bit_cast(h8_t, w);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float pf = exp2_fast(x[j >> 2][j & 3] - m_run);
-        const _Float16 p = (_Float16)pf;
-        ph[j] = p;
-        psum += kv_weights<KVF>() ? pf : (float)p;
-      }
+    for (int j = 0; j < 4; ++j) {
+      const float p0 = exp2_fast(x[j >> 1][2 * (j & 1)] - m_run), p1 = exp2_fast(x[j >> 1][2 * (j & 1) + 1] - m_run);
+      pw[j] = pack2<KVF>(p0, p1);
+      if constexpr (kv_weights<KVF>()) o_l[0] += p0 + p1;
     }
-    l_run += psum;
-    // V through LDS, one tile after the other in the same 16 rows (a wave's
+    const h8_t ph = __builtin_bit_cast(h8_t, pw);
+    if constexpr (!kv_weights<KVF>()) {
+      const uint32_t ones = pack2<KVF>(1.f, 1.f);
+      o_l = mfma16x32<KVF>(__builtin_bit_cast(h8_t, u4_t{ones, ones, ones, ones}), ph, o_l);
+    }
+    // V through LDS, one block after the other in the same 16 rows (a wave's
     // LDS accesses complete in order).
     h4_t vt[2][DT];
 #pragma unroll
@@ -286,23 +331,23 @@ __device__ __forceinline__ void wave_loop_mx4(const Phase1Args& a, const int32_t
       o[dt] = mfma16x32<KVF>(__builtin_shufflevector(vt[0][dt], vt[1][dt], 0, 1, 2, 3, 4, 5, 6, 7), ph, o[dt]);
   };
 
-  // This wave's pairs are wave, wave+nw, ...: the next pair's rows are in
-  // flight while one is computed.
+  // The next pair's rows are in flight while one is computed.
+  const int npair = (nblk + 1) >> 1;
   const int n_mine = wave < npair ? (npair - wave + nw - 1) / nw : 0;
   Tile ta, tb;
   if (n_mine > 0) {
     int it = 0;
-    fetch_ids(wave);
-    load(ta, wave);
+    fetch_ids();
+    load(ta);
     load_q();
     for (; it + 2 < n_mine; it += 2) {
-      load(tb, wave + (it + 1) * nw);
+      load(tb);
       compute(ta, wave + it * nw);
-      load(ta, wave + (it + 2) * nw);
+      load(ta);
       compute(tb, wave + (it + 1) * nw);
     }
     if (it + 1 < n_mine) {
-      load(tb, wave + (it + 1) * nw);
+      load(tb);
       compute(ta, wave + it * nw);
       compute(tb, wave + (it + 1) * nw);
     } else {
@@ -310,11 +355,13 @@ __device__ __forceinline__ void wave_loop_mx4(const Phase1Args& a, const int32_t
     }
   }
 
-  float l_tot = l_run + shfl_xor_f(l_run, 16);
-  l_tot += shfl_xor_f(l_tot, 32);
+  if constexpr (kv_weights<KVF>()) {
+    o_l[0] += shfl_xor_f(o_l[0], 16);
+    o_l[0] += shfl_xor_f(o_l[0], 32);
+  }
   if (row_ok) {
-    if (g == 0) sm_ml[wave * 16 + r16] = make_float2(m_run, l_tot);
-    float* dst = sm_o + (wave * a.gqa + r16) * wave_row_floats<D>() + 4 * g;
+    if (g == 0) sm_ml[slot * 16 + r16] = make_float2(m_run, o_l[0]);
+    float* dst = sm_o + (slot * a.gqa + r16) * wave_row_floats<D>() + 4 * g;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f4_t*>(dst + dt * 16) = o[dt];
   }

@@ -1,31 +1,50 @@
-// pa_mx4.hip - the per-unit decode kernel over MX4 caches (pa_mx4.h).
+// pa_mx4.hip - the decode kernels over MX4 caches (pa_mx4.h).
 #include "pa_ext.h"
 #include "pa_phase1.h"
+#include "pa_range_kernel.h"
 
 namespace pad {
 
+template <int D, int MODE, int KVF>
+__global__ __launch_bounds__((range_waves<D, KVF>() * 64))
+    __attribute__((amdgpu_waves_per_eu((range_waves<D, KVF>() / 4)))) void pad_mx4_range_kernel(const RangeArgs) {
+  range_kernel<D, MODE, KVF>();
+}
+
+template <int D, int MODE, int KVF>
+static hipError_t launch_one(const RangeArgs& a, bool range, dim3 grid, int nw, size_t lds, hipStream_t st) {
+  if (!range) return launch_p1<D, MODE, 0, 0, KVF>(a, grid, nw, lds, st);
+  hipLaunchKernelGGL((pad_mx4_range_kernel<D, MODE, KVF>), dim3(a.groups), dim3(nw * 64), lds, st, a);
+  return hipGetLastError();
+}
+
+// Uniform mode addresses a block's rows with 32-bit offsets.
 template <int D, int KVF>
-static hipError_t launch_dim(const Phase1Args& a, dim3 grid, int nw, size_t lds, hipStream_t st) {
-  if (a.ps % kBlockTokens == 0) return launch_p1<D, kModeUniform, 0, 0, KVF>(a, grid, nw, lds, st);
-  return launch_p1<D, kModeGeneric, 0, 0, KVF>(a, grid, nw, lds, st);
+static hipError_t launch_dim(const RangeArgs& a, bool range, dim3 grid, int nw, size_t lds, hipStream_t st) {
+  const int64_t far = 15 * (a.sks | a.svs | a.skss | a.svss);
+  if (a.ps % kBlockTokens == 0 && far < (1ll << 30))
+    return launch_one<D, kModeUniform, KVF>(a, range, grid, nw, lds, st);
+  return launch_one<D, kModeGeneric, KVF>(a, range, grid, nw, lds, st);
 }
 
 template <int KVF>
-static hipError_t launch_format(const Phase1Args& a, int head_dim, dim3 grid, int nw, size_t lds, hipStream_t st) {
+static hipError_t launch_format(const RangeArgs& a, bool range, int head_dim, dim3 grid, int nw, size_t lds,
+                                hipStream_t st) {
   switch (head_dim) {
-    case 64: return launch_dim<64, KVF>(a, grid, nw, lds, st);
-    case 128: return launch_dim<128, KVF>(a, grid, nw, lds, st);
-    case 256: return launch_dim<256, KVF>(a, grid, nw, lds, st);
+    case 64: return launch_dim<64, KVF>(a, range, grid, nw, lds, st);
+    case 128: return launch_dim<128, KVF>(a, range, grid, nw, lds, st);
+    case 256: return launch_dim<256, KVF>(a, range, grid, nw, lds, st);
     default: return hipErrorInvalidValue;
   }
 }
 
-hipError_t launch_mx4(const Phase1Args& a, int head_dim, int kvf, dim3 grid, int nw, size_t lds, hipStream_t st) {
+hipError_t launch_mx4(const RangeArgs& a, bool range, int head_dim, int kvf, dim3 grid, int nw, size_t lds,
+                      hipStream_t st) {
   switch (kvf) {
-    case kKvMx4: return launch_format<kKvMx4>(a, head_dim, grid, nw, lds, st);
-    case kKvMx4B: return launch_format<kKvMx4B>(a, head_dim, grid, nw, lds, st);
-    case kKvMx4 | kKvWeights: return launch_format<kKvMx4 | kKvWeights>(a, head_dim, grid, nw, lds, st);
-    case kKvMx4B | kKvWeights: return launch_format<kKvMx4B | kKvWeights>(a, head_dim, grid, nw, lds, st);
+    case kKvMx4: return launch_format<kKvMx4>(a, range, head_dim, grid, nw, lds, st);
+    case kKvMx4B: return launch_format<kKvMx4B>(a, range, head_dim, grid, nw, lds, st);
+    case kKvMx4 | kKvWeights: return launch_format<kKvMx4 | kKvWeights>(a, range, head_dim, grid, nw, lds, st);
+    case kKvMx4B | kKvWeights: return launch_format<kKvMx4B | kKvWeights>(a, range, head_dim, grid, nw, lds, st);
     default: return hipErrorInvalidValue;
   }
 }

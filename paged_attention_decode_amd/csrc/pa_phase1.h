@@ -34,29 +34,6 @@ struct KVTile {
   HVec<D * ES / 64> v[4];
 };
 
-// Scores of kKvWeights calls: row `row` of the unit's, by token.
-__device__ __forceinline__ float* logits_of(const Phase1Args& a, int b, int kvh, int row) {
-  return a.logits + (((int64_t)b * a.hkv + kvh) * a.gqa + row) * a.slog;
-}
-
-// The first n of four consecutive scores (rows start at any token, so the
-// vector store is aligned to a float only).
-__device__ __forceinline__ void store_logits(float* p, const float (&x)[4], int n) {
-  typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
-  if (n >= 4) {
-    *reinterpret_cast<f4u_t*>(p) = f4u_t{x[0], x[1], x[2], x[3]};
-  } else {
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (i < n) p[i] = x[i];
-  }
-}
-
-// log2 of a row's normaliser: m in base-2 units, l the sum of 2^(score - m).
-__device__ __forceinline__ void store_lse(const Phase1Args& a, int b, int kvh, int row, float m, float l) {
-  a.lse[((int64_t)b * a.hkv + kvh) * a.gqa + row] = m + __builtin_amdgcn_logf(l);
-}
-
 // Engine 0: MFMA 16x16x16 f16 tiles, two blocks in flight per wave (the
 // loads of block j+nw are issued before block j is computed).
 template <int D, int MODE, int KVF = kKvF16>
@@ -860,7 +837,7 @@ __device__ __forceinline__ bool worklist_item(const Phase1Args& a, int g, int G,
 // not fit 168 registers without one VGPR spilled to scratch; so do the
 // bfloat16 sub-page modes of head_dim 128 (2 VGPRs spilled at page size 4).
 constexpr int phase1_waves_per_simd(int d, int engine, int mode, int kvf) {
-  if ((kvf & 15) >= kKvMx4) return mx4_waves_per_simd(d, (kvf & kKvWeights) != 0);
+  if ((kvf & 15) >= kKvMx4) return mx4_waves_per_simd(d);
   const bool wide = d == 128 && (mode == 0 || ((kvf == kKvBF16 || kvf == kKvE4M3B || kvf == kKvE5M2B) &&
                                                  mode >= kModeSubpage) || (kvf & kKvWeights));
   return engine == 0 ? (d <= 128 ? (wide ? 2 : 3) : 1) : 1;
@@ -982,8 +959,8 @@ void pad_phase1_kernel(const Phase1Args a) {
   const int nblk = (t_end - t_begin + kBlockTokens - 1) / kBlockTokens;
 
   if constexpr (kv_is_mx4<KVF>()) {
-    wave_loop_mx4<D, MODE, KVF>(a, it.ids_row, it.ids_stride, b, kvh, t_begin, t_end, nblk, wave, nw, lane, sm_ml,
-                                sm_o, k_stage_all + wave * k_stage_bytes<D>());
+    wave_loop_mx4<D, MODE, KVF>(a, it.ids_row, it.ids_stride, b, kvh, t_begin, t_end, nblk, wave, nw, wave, lane,
+                                sm_ml, sm_o, k_stage_all + wave * k_stage_bytes<D>());
   } else if constexpr (ENGINE == 0) {
     wave_loop_mfma<D, MODE, KVF>(a, phys_first, it.ids_row, it.ids_stride, b, kvh, t_begin, t_end, nblk, wave,
                                  nw, lane, sm_ml, sm_o, k_stage_all + wave * k_stage_bytes<D>(),
@@ -1041,7 +1018,7 @@ void pad_phase1_kernel(const Phase1Args a) {
       for (int i = 0; i < 4; ++i) hv[i] = round16<KVF>(acc[i] * inv);
       *reinterpret_cast<h4_t*>(out_bh + (int64_t)row * a.soh + col) = hv;
       if constexpr (kv_weights<KVF>())
-        if (col == 0) store_lse(a, b, kvh, row, M, Ls);
+        if (col == 0) store_lse(a, b, kvh * gqa + row, M, Ls);
     } else {
       const uint32_t r = (uint32_t)(my_split * gqa + row);
       store_device(o_rsrc, (r * D + col) * 4u, acc);
@@ -1260,7 +1237,7 @@ void pad_phase1_kernel(const Phase1Args a) {
     for (int i = 0; i < 4; ++i) hv[i] = round16<KVF>(acc[i] * inv);
     *reinterpret_cast<h4_t*>(out_bh + (int64_t)row * a.soh + col) = hv;
     if constexpr (kv_weights<KVF>())
-      if (col == 0) store_lse(a, b, kvh, row, m, l);
+      if (col == 0) store_lse(a, b, kvh * gqa + row, m, l);
   }
   if (threadIdx.x == 0) atomicExch(unit_counter, 0);
   PAD_TL(lin, PAD_TL_MERGED);

@@ -895,10 +895,14 @@ torch::Tensor cache_decode(torch::Tensor q, torch::Tensor k_cache, torch::Tensor
   const int splits = num_splits.has_value() ? static_cast<int>(*num_splits) : 0;
   pad_decode_dims d;
   fill_dims(q, k_cache, v_cache, block_table, seq_lens, out, &d);
-  pad_decode_plan_t plan;
+  const bool bf16 = q.scalar_type() == at::kBFloat16;
+  const int format = mx4 ? (bf16 ? PAD_KV_MX4_BF16 : PAD_KV_MX4) : cache_format(q, k_cache, v_cache);
   const int cus = cached_cus(q.get_device());
-  int st = pad_decode_plan(&d, splits, cus, &plan);
+  pad_decode_plan_t plan;  // its scratch fields
+  std::memset(&plan, 0, sizeof(plan));
+  int st = pad_cache_scratch(&d, format, splits, cus, &plan.workspace_bytes, &plan.counters);
   TORCH_CHECK(st == PAD_OK, "pa_decode: ", pad_status_string(st));
+  plan.single_pass = plan.workspace_bytes == 0;
   hipStream_t stream = current_stream(q);
   pad_cache_call cc;
   std::memset(&cc, 0, sizeof(cc));
@@ -917,8 +921,7 @@ torch::Tensor cache_decode(torch::Tensor q, torch::Tensor k_cache, torch::Tensor
   c.scale = scale.has_value() ? static_cast<float>(*scale)
                               : static_cast<float>(1.0 / std::sqrt(static_cast<double>(desc.head_dim)));
   c.num_splits = splits;
-  const bool bf16 = q.scalar_type() == at::kBFloat16;
-  c.kv_format = mx4 ? (bf16 ? PAD_KV_MX4_BF16 : PAD_KV_MX4) : cache_format(q, k_cache, v_cache);
+  c.kv_format = format;
   c.k_scale = desc.k_scale;
   c.v_scale = desc.v_scale;
   cc.k_scales = desc.k_scales;
