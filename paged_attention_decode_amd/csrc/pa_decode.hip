@@ -452,7 +452,8 @@ static RangeShape range_shape(const pad_decode_dims* d, int num_splits, int num_
 #endif
   if (num_cus <= 0) num_cus = 256;
   const int64_t units = (int64_t)d->batch * d->num_kv_heads;
-  if (num_splits != 0 || engine != 0 || d->batch <= 0 || d->batch > kRangeMaxBatch || d->num_kv_heads == 2) return r;
+  if (num_splits != 0 || engine != 0 || d->batch <= 0 || d->batch > kRangeMaxBatch) return r;
+  if (d->num_kv_heads == 2 && !mx4) return r;
   r.nh_shift = d->num_kv_heads % 4 == 0 ? 2 : (d->num_kv_heads % 2 == 0 ? 1 : 0);
   // Rows of at most 128 bytes: 8 waves keep as many bytes in flight as 4 of
   // wider rows (fp8, 64 x [1, 8192]: 93.3 us with 8, 93.8 with 4; head_dim 64,
@@ -470,9 +471,17 @@ static RangeShape range_shape(const pad_decode_dims* d, int num_splits, int num_
   // [1, 4608] of 24/6 1.05), and so does head_dim 64 (9 x [1, 7264] 1.32).
   if (units * 4 <= num_cus || units * 2 == num_cus || latency_bound_shape(d, num_cus, csr)) return r;
   if (r.nh_shift == 2 && (r.nw == kMaxWaves / 2 ? units * 2 < num_cus : kv_bytes == 1 && units * 3 <= num_cus)) return r;
+  // MX4 rows are short: a per-unit workgroup's share of them does not pay for its
+  // fixed costs, so two kv heads take ranges as well, and groups of four from
+  // rows of 512 tokens (of 128) on.  us, per unit / ranges: 48 x [1, 4096] of 12/2
+  // 17.5 / 15.9, 66 23.2 / 18.1, 200 48.2 / 31.4 (33 13.4 / 15.8); 200 x [1, 512]
+  // of 32/8 45.2 / 26.5, full 35.7 / 31.5, 120 27.6 / 20.0 (120 x [1, 416] 16.9 /
+  // 19.2).
+  if (mx4 && units * 3 <= num_cus) return r;
+  const int64_t least_row = mx4 && r.nh_shift == 2 ? kRangeRowBytes * 2 / 3 : kRangeRowBytes;
   const int64_t page_bytes = ((int64_t)d->page_size * d->head_dim * (mx4 ? 1 : kv_bytes * 2)) << r.nh_shift;
   const int64_t row_bytes = plan_pages_per_seq(d, csr) * (((int64_t)d->page_size * d->head_dim * 4) << r.nh_shift);
-  if (row_bytes < kRangeRowBytes || (units >> r.nh_shift) * row_bytes < kRangeCallBytes) return r;
+  if (row_bytes < least_row || (units >> r.nh_shift) * row_bytes < kRangeCallBytes) return r;
   // Positions are counted in 32 bits (twice the pages at most, and unit_extra).
   if (d->batch * (2 * (int64_t)d->max_pages + 4096) > (1 << 30) / d->num_kv_heads) return r;
   // A work list holds a record per workgroup and two sequences per record.

@@ -106,9 +106,10 @@ __device__ __forceinline__ h4_t lds_read_transposed(const char* p) {
 // One wave's part of an item: tokens [t_begin, t_end) (t_begin on a page border,
 // nblk blocks of 16) of kv head kvh, of which the wave takes the pairs of blocks
 // wave, wave + nw, ...; its state goes to place `slot` of sm_ml and sm_o.
-// MODE: kModeUniform (a 16-token block lies in one page) or kModeGeneric (each
-// lane finds its own tokens' pages).  Strides are below 2^32 bytes, and in
-// uniform mode 15 rows apart are below 2^31 (the launcher sees to both).
+// MODE: kModeUniform (a 16-token block lies in one page, its rows next to each
+// other) or kModeGeneric (each lane finds its own tokens' pages).  Strides are
+// below 2^32 bytes, the scales' slot strides below 2^26 in uniform mode (the
+// launcher sees to both).
 template <int D, int MODE, int KVF>
 __device__ __forceinline__ void wave_loop_mx4(const Phase1Args& a, const int32_t* bt_row, int64_t ids_stride, int b,
                                               int kvh, int t_begin, int t_end, int nblk, int wave, int nw, int slot,
@@ -214,7 +215,7 @@ __device__ __forceinline__ void wave_loop_mx4(const Phase1Args& a, const int32_t
     } else {
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const HVec<CW> w = load_hvec_stream<CW>(reinterpret_cast<const _Float16*>(base + off + c * 64));
+        const HVec<CW> w = load_hvec<CW>(reinterpret_cast<const _Float16*>(base + off + c * 64));
 #pragma unroll
         for (int j = 0; j < CW; ++j) x.w[c * CW + j] = w.w[j];
       }

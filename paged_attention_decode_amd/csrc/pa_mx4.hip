@@ -18,11 +18,16 @@ static hipError_t launch_one(const RangeArgs& a, bool range, dim3 grid, int nw, 
   return hipGetLastError();
 }
 
-// Uniform mode addresses a block's rows with 32-bit offsets.
+// Uniform mode is for blocks whose rows lie next to each other: it streams them
+// (non-temporal loads).  Rows of several kv heads in one cache line are loaded
+// by each lane's own address and kept in the CU's cache, where the other heads'
+// waves find the rest of the line.  us, streamed / kept: heads next to each other
+// 64 x [1, 8192] of 32/8 89.4 / 85.3, 27 x [1, 4096] of 32/8 at head_dim 64, page
+// 1, 34.1 / 24.6; rows next to each other 56.3 / 63.1, 1 x 131072 31.1 / 34.0.
 template <int D, int KVF>
 static hipError_t launch_dim(const RangeArgs& a, bool range, dim3 grid, int nw, size_t lds, hipStream_t st) {
-  const int64_t far = 15 * (a.sks | a.svs | a.skss | a.svss);
-  if (a.ps % kBlockTokens == 0 && far < (1ll << 30))
+  const bool rows = a.sks == D / 2 && a.svs == D / 2 && (a.skss | a.svss) < (1 << 26);
+  if (a.ps % kBlockTokens == 0 && rows)
     return launch_one<D, kModeUniform, KVF>(a, range, grid, nw, lds, st);
   return launch_one<D, kModeGeneric, KVF>(a, range, grid, nw, lds, st);
 }
