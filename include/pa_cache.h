@@ -78,8 +78,8 @@ int pad_cache_decode(const pad_cache_call* call, const pad_decode_dims* dims,
                      void* stream);
 
 /* One layer's caches.  kv_format: PAD_KV_FP16, PAD_KV_BF16, PAD_KV_FP8_E4M3FN,
- * PAD_KV_FP8_E5M2 or PAD_KV_MX4; strides (page, slot, kv head) in elements of
- * the cache, which are bytes of codes for MX4.  k_scale, v_scale: fp8 caches hold
+ * PAD_KV_FP8_E5M2 or PAD_KV_MX4; strides (page, slot, kv head; 0 to 2^32 - 1) in
+ * elements of the cache, which are bytes of codes for MX4.  k_scale, v_scale: fp8 caches hold
  * K / k_scale and V / v_scale.  k_scales, v_scales: MX4 only.  weights and
  * positions may be NULL in append and read, not in evict. */
 typedef struct pad_kv_cache {
@@ -101,7 +101,7 @@ typedef struct pad_kv_cache {
   float v_scale;
 } pad_kv_cache;
 
-/* Rows [tokens, num_kv_heads, head_dim] of an append or a read: fp16, or
+/* Rows [tokens, num_kv_heads, head_dim] (fewer than 2^31 rows) of an append or a read: fp16, or
  * bfloat16 (bf16 = 1), with strides of token and kv head in elements (rows
  * contiguous and 16-byte aligned).  slots: page * page_size + slot of every
  * token, int64 (slots64 = 1) or int32, contiguous. */

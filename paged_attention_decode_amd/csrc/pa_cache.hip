@@ -13,9 +13,11 @@ namespace pad {
 typedef float f2_t __attribute__((ext_vector_type(2)));
 
 // ---------------------------------------------------------------------------
-// Append and read.  A thread has eight elements of a row (16 bytes of 16-bit
-// values); the four lanes of an MX4 block find its largest value together.  Bound
-// by memory: the rows are read (or written) once, the cache's the other way.
+// Append and read.  A thread has eight elements of a row of K and of V (16 bytes
+// of 16-bit values each); the four lanes of an MX4 block find its largest value
+// together.  Bound by memory: the rows are read (or written) once, the cache's
+// the other way.  (One of K and V a thread and 64-bit index arithmetic: 16000
+// MX4 rows of 8 heads 23.4 + 19.0 us; so 20.8 + 17.0.)
 // ---------------------------------------------------------------------------
 constexpr int kRows16 = 0, kRowsE4M3 = 1, kRowsE5M2 = 2, kRowsMx4 = 3;  // kinds of cache rows
 
@@ -24,27 +26,55 @@ struct RowArgs {
   pad_kv_rows r;
   const float* token_weights;
   const int32_t* token_positions;
-  int64_t work;  // tokens * kv heads * (head_dim / 8)
-  int row8;      // head_dim / 8
-  int ps_shift;
+  uint32_t rows;  // tokens * kv heads
+  int row8;       // head_dim / 8
+  int row8_shift, ps_shift, head_shift;  // log2 where a power of two, else -1
+  int same;       // K and V (and their scales) have the same strides
 };
 
-__device__ __forceinline__ int64_t slot_of(const RowArgs& a, int64_t token) {
+__device__ __forceinline__ uint32_t divide(uint32_t x, int shift, uint32_t by) { return shift >= 0 ? x >> shift : x / by; }
+
+__device__ __forceinline__ int64_t slot_of(const RowArgs& a, uint32_t token) {
   return a.r.slots64 ? static_cast<const int64_t*>(a.r.slots)[token] : static_cast<const int32_t*>(a.r.slots)[token];
 }
 
+// The thread's row and eight elements of it; false past the last row.
+struct RowPart {
+  uint32_t row, token, h, e8;
+};
+__device__ __forceinline__ bool row_part(const RowArgs& a, RowPart& p) {
+  // Workgroups have whole rows (256 is a multiple of row8 but at head_dim 96:
+  // 252 threads of 21 rows).
+  const uint32_t per = a.row8_shift >= 0 ? 256u >> a.row8_shift : 256u / (uint32_t)a.row8;
+  const uint32_t sub = divide(threadIdx.x, a.row8_shift, a.row8);
+  if (sub >= per) return false;
+  p.row = blockIdx.x * per + sub;
+  p.e8 = threadIdx.x - sub * a.row8;
+  p.token = divide(p.row, a.head_shift, a.c.num_kv_heads);
+  p.h = p.row - p.token * a.c.num_kv_heads;
+  return p.row < a.rows;
+}
+
+// Strides are below 2^32 (check_cache), so that each product is one instruction.
+__device__ __forceinline__ uint64_t offset_of(const int64_t* st, uint32_t page, uint32_t at, uint32_t h) {
+  return (uint64_t)page * (uint32_t)st[0] + (uint64_t)at * (uint32_t)st[1] + (uint64_t)h * (uint32_t)st[2];
+}
+
 // Page and place of a slot; false for one outside the cache.
-__device__ __forceinline__ bool place_of(const RowArgs& a, int64_t s, int64_t& page, int64_t& at) {
+__device__ __forceinline__ bool place_of(const RowArgs& a, int64_t s, uint32_t& page, uint32_t& at) {
   if (s < 0) return false;
+  int64_t p;
   if (a.ps_shift >= 0) {
-    page = s >> a.ps_shift;
+    p = s >> a.ps_shift;
   } else if (s < (1ll << 32)) {
-    page = (uint32_t)s / (uint32_t)a.c.page_size;
+    p = (uint32_t)s / (uint32_t)a.c.page_size;
   } else {
-    page = s / a.c.page_size;
+    p = s / a.c.page_size;
   }
-  at = s - page * a.c.page_size;
-  return page < a.c.num_pages;
+  if (p >= a.c.num_pages) return false;
+  page = (uint32_t)p;
+  at = (uint32_t)(s - p * a.c.page_size);
+  return true;
 }
 
 template <bool BF16>
@@ -99,26 +129,11 @@ __device__ __forceinline__ uint32_t fp8x4(const float* x, float scale) {
   return (uint32_t)w;
 }
 
+// One row's eight elements into a cache, at element (byte) `off` of the row's place.
 template <int KIND, bool BF16>
-__global__ __launch_bounds__(256) void pad_append_kernel(const RowArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const bool is_v = blockIdx.y != 0;
-  // Rows have whole groups of four threads, so a block's lanes live or leave
-  // together.
-  if (i >= a.work) return;
-  const int64_t row = i / a.row8;
-  const int e8 = (int)(i - row * a.row8);
-  const int64_t token = row / a.c.num_kv_heads;
-  const int h = (int)(row - token * a.c.num_kv_heads);
-  const _Float16* src = static_cast<const _Float16*>(is_v ? a.r.v : a.r.k) +
-                        token * (is_v ? a.r.v_stride[0] : a.r.k_stride[0]) +
-                        (int64_t)h * (is_v ? a.r.v_stride[1] : a.r.k_stride[1]) + e8 * 8;
-  const u4_t w = __builtin_nontemporal_load(reinterpret_cast<const u4_t*>(src));
-  int64_t page, at;
-  if (!place_of(a, slot_of(a, token), page, at)) return;
-  const int64_t* st = is_v ? a.c.v_stride : a.c.k_stride;
-  const int64_t off = page * st[0] + at * st[1] + (int64_t)h * st[2];
-  char* base = static_cast<char*>(is_v ? a.c.v : a.c.k);
+__device__ __forceinline__ void store_part(u4_t w, void* cache, uint8_t* scales, uint64_t off, uint64_t scale_off,
+                                           float scale, uint32_t e8) {
+  char* base = static_cast<char*>(cache);
   if constexpr (KIND == kRows16) {
     *reinterpret_cast<u4_t*>(base + (off + e8 * 8) * 2) = w;
   } else {
@@ -128,97 +143,140 @@ __global__ __launch_bounds__(256) void pad_append_kernel(const RowArgs a) {
       uint32_t top = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
-      top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
-      top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
+      top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, false));  // the block's four lanes
+      top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, false));
       const int e = (int)(top >> 23);  // biased; 255: NaN or infinity
       const uint32_t s = e == 255 ? 255u : (uint32_t)max(e - 2, 0);
       // v_cvt_scalef32_pk_fp4_f32 divides by the scale, rounds to nearest even
       // and saturates (exponent byte 0 stands for 2^-127).
-      const float scale = __uint_as_float(s << 23);
+      const float by = __uint_as_float(s << 23);
       uint32_t codes = 0;
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], scale, 0);
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], scale, 1);
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], scale, 2);
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], scale, 3);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], by, 0);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], by, 1);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], by, 2);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], by, 3);
       *reinterpret_cast<uint32_t*>(base + off + e8 * 4) = e == 255 ? 0u : codes;
-      if ((e8 & 3) == 0) {
-        const int64_t* ss = is_v ? a.c.vs_stride : a.c.ks_stride;
-        (is_v ? a.c.v_scales : a.c.k_scales)[page * ss[0] + at * ss[1] + (int64_t)h * ss[2] + (e8 >> 2)] = (uint8_t)s;
-      }
+      if ((e8 & 3) == 0) scales[scale_off + (e8 >> 2)] = (uint8_t)s;
     } else {
-      const float scale = is_v ? a.c.v_scale : a.c.k_scale;
       *reinterpret_cast<u2_t*>(base + off + e8 * 8) = u2_t{fp8x4<KIND>(x, scale), fp8x4<KIND>(x + 4, scale)};
     }
   }
-  if (e8 == 0) {
-    if (!is_v && a.c.weights)
-      a.c.weights[page * a.c.w_stride[0] + at * a.c.w_stride[1] + (int64_t)h * a.c.w_stride[2]] =
-          a.token_weights ? a.token_weights[row] : 0.f;
-    if (is_v && a.c.positions)
-      a.c.positions[page * a.c.p_stride[0] + at * a.c.p_stride[1] + (int64_t)h * a.c.p_stride[2]] =
-          a.token_positions[token];
+}
+
+template <int KIND, bool BF16>
+__global__ __launch_bounds__(256) void pad_append_kernel(const RowArgs a) {
+  RowPart p;
+  if (!row_part(a, p)) return;
+  const _Float16* ks = static_cast<const _Float16*>(a.r.k) + (int64_t)p.token * a.r.k_stride[0] +
+                       (int64_t)p.h * a.r.k_stride[1] + p.e8 * 8;
+  const _Float16* vs = static_cast<const _Float16*>(a.r.v) + (int64_t)p.token * a.r.v_stride[0] +
+                       (int64_t)p.h * a.r.v_stride[1] + p.e8 * 8;
+  const u4_t k = __builtin_nontemporal_load(reinterpret_cast<const u4_t*>(ks));
+  const u4_t v = __builtin_nontemporal_load(reinterpret_cast<const u4_t*>(vs));
+  // A row's threads (and so an MX4 block's four lanes) go on or leave together.
+  uint32_t page, at;
+  if (!place_of(a, slot_of(a, p.token), page, at)) return;
+  const uint64_t koff = offset_of(a.c.k_stride, page, at, p.h);
+  const uint64_t voff = a.same ? koff : offset_of(a.c.v_stride, page, at, p.h);
+  uint64_t ksoff = 0, vsoff = 0;
+  if constexpr (KIND == kRowsMx4) {
+    ksoff = offset_of(a.c.ks_stride, page, at, p.h);
+    vsoff = a.same ? ksoff : offset_of(a.c.vs_stride, page, at, p.h);
+  }
+  store_part<KIND, BF16>(k, a.c.k, a.c.k_scales, koff, ksoff, a.c.k_scale, p.e8);
+  store_part<KIND, BF16>(v, a.c.v, a.c.v_scales, voff, vsoff, a.c.v_scale, p.e8);
+  if (p.e8 == 0) {
+    if (a.c.weights)
+      a.c.weights[offset_of(a.c.w_stride, page, at, p.h)] = a.token_weights ? a.token_weights[p.row] : 0.f;
+    if (a.c.positions) a.c.positions[offset_of(a.c.p_stride, page, at, p.h)] = a.token_positions[p.token];
+  }
+}
+
+// Eight elements of a row as 16-bit values; the cache's words are loaded first
+// (load_part), so that K's and V's are in flight together.
+template <int KIND>
+struct Part {
+  u4_t w;
+  uint32_t scale;
+};
+template <int KIND>
+__device__ __forceinline__ Part<KIND> load_part(const void* cache, const uint8_t* scales, uint64_t off,
+                                                uint64_t scale_off, uint32_t e8) {
+  const char* base = static_cast<const char*>(cache);
+  Part<KIND> p = {};
+  if constexpr (KIND == kRows16) {
+    p.w = *reinterpret_cast<const u4_t*>(base + (off + e8 * 8) * 2);
+  } else if constexpr (KIND == kRowsMx4) {
+    p.w[0] = *reinterpret_cast<const uint32_t*>(base + off + e8 * 4);
+    p.scale = scales[scale_off + (e8 >> 2)];
+  } else {
+    const u2_t w = *reinterpret_cast<const u2_t*>(base + off + e8 * 8);
+    p.w[0] = w[0];
+    p.w[1] = w[1];
+  }
+  return p;
+}
+template <int KIND, bool BF16>
+__device__ __forceinline__ u4_t values_of(const Part<KIND>& p, float scale) {
+  float x[8];
+  if constexpr (KIND == kRows16) {
+    return p.w;
+  } else if constexpr (KIND == kRowsMx4) {
+    const float by = __uint_as_float(p.scale << 23);
+    const uint32_t w = p.w[0];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f2_t y = j == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, by, 0)
+                     : j == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, by, 1)
+                     : j == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, by, 2)
+                              : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, by, 3);
+      x[2 * j] = y.x;
+      x[2 * j + 1] = y.y;
+    }
+    return pack8<BF16>(x);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      f2_t lo, hi;
+      if constexpr (KIND == kRowsE4M3) {
+        lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)p.w[j], false);
+        hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)p.w[j], true);
+      } else {
+        lo = __builtin_amdgcn_cvt_pk_f32_bf8((int)p.w[j], false);
+        hi = __builtin_amdgcn_cvt_pk_f32_bf8((int)p.w[j], true);
+      }
+      x[4 * j] = lo.x * scale;
+      x[4 * j + 1] = lo.y * scale;
+      x[4 * j + 2] = hi.x * scale;
+      x[4 * j + 3] = hi.y * scale;
+    }
+    return pack8<BF16>(x);
   }
 }
 
 template <int KIND, bool BF16>
 __global__ __launch_bounds__(256) void pad_read_kernel(const RowArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const bool is_v = blockIdx.y != 0;
-  if (i >= a.work) return;
-  const int64_t row = i / a.row8;
-  const int e8 = (int)(i - row * a.row8);
-  const int64_t token = row / a.c.num_kv_heads;
-  const int h = (int)(row - token * a.c.num_kv_heads);
-  _Float16* dst = static_cast<_Float16*>(is_v ? a.r.v : a.r.k) + token * (is_v ? a.r.v_stride[0] : a.r.k_stride[0]) +
-                  (int64_t)h * (is_v ? a.r.v_stride[1] : a.r.k_stride[1]) + e8 * 8;
-  int64_t page, at;
-  u4_t out = (u4_t)0u;
-  if (place_of(a, slot_of(a, token), page, at)) {
-    const int64_t* st = is_v ? a.c.v_stride : a.c.k_stride;
-    const int64_t off = page * st[0] + at * st[1] + (int64_t)h * st[2];
-    const char* base = static_cast<const char*>(is_v ? a.c.v : a.c.k);
-    if constexpr (KIND == kRows16) {
-      out = *reinterpret_cast<const u4_t*>(base + (off + e8 * 8) * 2);
-    } else if constexpr (KIND == kRowsMx4) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(base + off + e8 * 4);
-      const int64_t* ss = is_v ? a.c.vs_stride : a.c.ks_stride;
-      const uint32_t s = (is_v ? a.c.v_scales
-                               : a.c.k_scales)[page * ss[0] + at * ss[1] + (int64_t)h * ss[2] + (e8 >> 2)];
-      const float scale = __uint_as_float(s << 23);
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f2_t p = j == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0)
-                       : j == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1)
-                       : j == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 2)
-                                : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 3);
-        x[2 * j] = p.x;
-        x[2 * j + 1] = p.y;
-      }
-      out = pack8<BF16>(x);
-    } else {
-      const u2_t w = *reinterpret_cast<const u2_t*>(base + off + e8 * 8);
-      const float scale = is_v ? a.c.v_scale : a.c.k_scale;
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        f2_t lo, hi;
-        if constexpr (KIND == kRowsE4M3) {
-          lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j], false);
-          hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j], true);
-        } else {
-          lo = __builtin_amdgcn_cvt_pk_f32_bf8((int)w[j], false);
-          hi = __builtin_amdgcn_cvt_pk_f32_bf8((int)w[j], true);
-        }
-        x[4 * j] = lo.x * scale;
-        x[4 * j + 1] = lo.y * scale;
-        x[4 * j + 2] = hi.x * scale;
-        x[4 * j + 3] = hi.y * scale;
-      }
-      out = pack8<BF16>(x);
+  RowPart p;
+  if (!row_part(a, p)) return;
+  u4_t k = (u4_t)0u, v = (u4_t)0u;
+  uint32_t page, at;
+  if (place_of(a, slot_of(a, p.token), page, at)) {
+    const uint64_t koff = offset_of(a.c.k_stride, page, at, p.h);
+    const uint64_t voff = a.same ? koff : offset_of(a.c.v_stride, page, at, p.h);
+    uint64_t ksoff = 0, vsoff = 0;
+    if constexpr (KIND == kRowsMx4) {
+      ksoff = offset_of(a.c.ks_stride, page, at, p.h);
+      vsoff = a.same ? ksoff : offset_of(a.c.vs_stride, page, at, p.h);
     }
+    const Part<KIND> kp = load_part<KIND>(a.c.k, a.c.k_scales, koff, ksoff, p.e8);
+    const Part<KIND> vp = load_part<KIND>(a.c.v, a.c.v_scales, voff, vsoff, p.e8);
+    k = values_of<KIND, BF16>(kp, a.c.k_scale);
+    v = values_of<KIND, BF16>(vp, a.c.v_scale);
   }
-  __builtin_nontemporal_store(out, reinterpret_cast<u4_t*>(dst));
+  _Float16* kd = static_cast<_Float16*>(a.r.k) + (int64_t)p.token * a.r.k_stride[0] + (int64_t)p.h * a.r.k_stride[1];
+  _Float16* vd = static_cast<_Float16*>(a.r.v) + (int64_t)p.token * a.r.v_stride[0] + (int64_t)p.h * a.r.v_stride[1];
+  __builtin_nontemporal_store(k, reinterpret_cast<u4_t*>(kd + p.e8 * 8));
+  __builtin_nontemporal_store(v, reinterpret_cast<u4_t*>(vd + p.e8 * 8));
 }
 
 // ---------------------------------------------------------------------------
@@ -632,6 +690,12 @@ static int check_cache(const pad_kv_cache* c) {
   if ((kind == kRowsE4M3 || kind == kRowsE5M2) &&
       (!(c->k_scale > 0.f) || !(c->v_scale > 0.f) || c->k_scale > 1e30f || c->v_scale > 1e30f))
     return PAD_ERR_KV_FORMAT;
+  // Offsets are sums of 32 by 32 bit products.
+  const int64_t* strides[] = {c->k_stride, c->v_stride, c->ks_stride, c->vs_stride, c->w_stride, c->p_stride};
+  const bool used[] = {true, true, kind == kRowsMx4, kind == kRowsMx4, c->weights != nullptr, c->positions != nullptr};
+  for (int j = 0; j < 6; ++j)
+    for (int i = 0; used[j] && i < 3; ++i)
+      if (strides[j][i] < 0 || strides[j][i] > UINT32_MAX) return PAD_ERR_STRIDE;
   const int need = kind == kRows16 ? 16 : 8;
   return row_alignment(c) < need ? PAD_ERR_ALIGNMENT : PAD_OK;
 }
@@ -643,9 +707,7 @@ static int check_rows(const pad_kv_cache* c, const pad_kv_rows* r) {
   if (r->tokens < 0) return PAD_ERR_INVALID_SHAPE;
   if (r->tokens == 0) return PAD_OK;
   if (!r->k || !r->v || !r->slots) return PAD_ERR_NULL_POINTER;
-  // A grid holds 2^31 - 1 workgroups of 256 threads.
-  if (r->tokens > ((int64_t)INT32_MAX * 256) / ((int64_t)c->num_kv_heads * (c->head_dim / 8)))
-    return PAD_ERR_INVALID_SHAPE;
+  if (r->tokens > INT32_MAX / c->num_kv_heads) return PAD_ERR_INVALID_SHAPE;  // rows are counted in 32 bits
   if ((((uintptr_t)r->k | (uintptr_t)r->v) & 15u) != 0 ||
       ((r->k_stride[0] | r->k_stride[1] | r->v_stride[0] | r->v_stride[1]) & 7) != 0)
     return PAD_ERR_ALIGNMENT;
@@ -655,7 +717,8 @@ static int check_rows(const pad_kv_cache* c, const pad_kv_rows* r) {
 
 template <template <int, bool> class K>
 static void launch_rows(const RowArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)((a.work + 255) / 256), 2);
+  const uint32_t per = 256u / (uint32_t)a.row8;
+  const dim3 grid((a.rows + per - 1) / per);
   const bool bf16 = a.r.bf16 != 0;
   switch (row_kind(a.c.kv_format)) {
     case kRows16: K<kRows16, false>::launch(a, grid, st); break;  // moved as bits
@@ -683,8 +746,14 @@ static RowArgs row_args(const pad_kv_cache* c, const pad_kv_rows* r) {
   a.c = *c;
   a.r = *r;
   a.row8 = c->head_dim / 8;
-  a.work = r->tokens * c->num_kv_heads * a.row8;
+  a.rows = (uint32_t)(r->tokens * c->num_kv_heads);
+  a.row8_shift = shift_of(a.row8);
   a.ps_shift = shift_of(c->page_size);
+  a.head_shift = shift_of(c->num_kv_heads);
+  a.same = 1;
+  for (int i = 0; i < 3; ++i)
+    if (c->k_stride[i] != c->v_stride[i] || (row_kind(c->kv_format) == kRowsMx4 && c->ks_stride[i] != c->vs_stride[i]))
+      a.same = 0;
   return a;
 }
 

@@ -503,23 +503,35 @@ __device__ __forceinline__ void fp8x4_to_16x4(uint32_t w, uint32_t& lo, uint32_t
 template <int D>
 constexpr bool q_in_lds() { return D >= 256; }
 
-// Scores of kKvWeights calls: those of row `row` of kv head kvh, by token.
-__device__ __forceinline__ float* logits_of(const Phase1Args& a, int b, int kvh, int row) {
-  return a.logits + ((int64_t)b * a.hq + kvh * a.gqa + row) * a.slog;
-}
-
-// The first n of four consecutive scores (rows start at any token, so the
-// vector store is aligned to a float only).
-__device__ __forceinline__ void store_logits(float* p, const float (&x)[4], int n) {
-  typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
-  if (n >= 4) {
-    *reinterpret_cast<f4u_t*>(p) = f4u_t{x[0], x[1], x[2], x[3]};
-  } else {
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (i < n) p[i] = x[i];
+// Scores of kKvWeights calls: those of kv head kvh's rows, slog floats each, as a
+// buffer (below 2^32 bytes, which the launcher sees to).  Stores past its end are dropped,
+// so rows that do not exist need no branch: one around the stores kept the
+// compiler from waiting for the loads before them alone.
+struct Logits {
+  __amdgpu_buffer_rsrc_t r;
+  uint32_t row;  // the lane's row, or past the end
+  __device__ __forceinline__ Logits(const Phase1Args& a, int b, int kvh, int r16) {
+    const uint32_t bytes = (uint32_t)(a.gqa * a.slog * 4);
+    r = make_rsrc(a.logits + ((int64_t)b * a.hq + kvh * a.gqa) * a.slog, bytes);
+    row = r16 < a.gqa ? (uint32_t)r16 * (uint32_t)a.slog * 4u : 0xffffffffu;
   }
-}
+  // Four consecutive scores from token t on, of which those below t_end are
+  // written; whole: all of the wave's are.
+  __device__ __forceinline__ void store(int t, const float (&x)[4], int t_end, bool whole) const {
+    const uint32_t off = row == 0xffffffffu ? 0xfffffff0u : row + (uint32_t)t * 4u;
+    if (whole) {
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i4_t, f4_t{x[0], x[1], x[2], x[3]}), r, off, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[i]), r, t + i < t_end ? off + 4u * i : 0xfffffff0u, 0, 0);
+    }
+  }
+};
+
+struct NoLogits {
+  __device__ __forceinline__ NoLogits(const Phase1Args&, int, int, int) {}
+};
 
 // log2 of a query head's normaliser: m in base-2 units, l the sum of 2^(score - m).
 __device__ __forceinline__ void store_lse(const Phase1Args& a, int b, int head, float m, float l) {

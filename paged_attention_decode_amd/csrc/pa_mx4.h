@@ -20,6 +20,8 @@
 #ifndef PA_MX4_H_
 #define PA_MX4_H_
 
+#include <type_traits>
+
 #include "pa_device.h"
 
 namespace pad {
@@ -141,8 +143,7 @@ __device__ __forceinline__ void wave_loop_mx4(const Phase1Args& a, const int32_t
   // Row sums of P from one more matrix step with an operand of ones; where the
   // caller gets the weights, which are unrounded, a lane's own sum.
   f4_t o_l = (f4_t)0.f;
-  float* logit_row = nullptr;
-  if constexpr (kv_weights<KVF>()) logit_row = logits_of(a, b, kvh, row_ok ? r16 : 0);
+  const std::conditional_t<kv_weights<KVF>(), Logits, NoLogits> logits(a, b, kvh, r16);
 
   const char* k_head = reinterpret_cast<const char*>(a.k) + (int64_t)kvh * a.skh;
   const char* v_head = reinterpret_cast<const char*>(a.v) + (int64_t)kvh * a.svh;
@@ -280,10 +281,7 @@ __device__ __forceinline__ void wave_loop_mx4(const Phase1Args& a, const int32_t
     }
     if constexpr (kv_weights<KVF>()) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int tk = t0 + 16 * u + 4 * g;
-        store_logits(logit_row + tk, x[u], row_ok ? t_end - tk : 0);
-      }
+      for (int u = 0; u < 2; ++u) logits.store(t0 + 16 * u + 4 * g, x[u], t_end, t0 + 32 <= t_end);
     }
     float bm = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                      fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));

@@ -8,6 +8,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "pa_device.h"
 #include "pa_decode_timeline.h"  // PAD_TL_* constants
 #include "pa_mx4.h"
@@ -122,8 +124,7 @@ __device__ __forceinline__ void wave_loop_mfma(const Phase1Args& a, int phys_fir
 
   const char* k_head = reinterpret_cast<const char*>(a.k) + (int64_t)kvh * a.skh * ES;
   const char* v_head = reinterpret_cast<const char*>(a.v) + (int64_t)kvh * a.svh * ES;
-  float* logit_row = nullptr;
-  if constexpr (kv_weights<KVF>()) logit_row = logits_of(a, b, kvh, row_ok ? r16 : 0);
+  const std::conditional_t<kv_weights<KVF>(), Logits, NoLogits> logits(a, b, kvh, r16);
   // Lane byte offsets inside a 16-token slab of one page (loop invariant).
   // K and V are both read as whole token rows: lane (g, r16) reads row
   // 4g+i, segments at head_dim r16*2*SEG (+ D/NSEG), so one load
@@ -293,7 +294,7 @@ __device__ __forceinline__ void wave_loop_mfma(const Phase1Args& a, int phys_fir
         if (!valid) t.v[i].zero();  // stale cache slots may hold NaN/Inf
       }
     }
-    if constexpr (kv_weights<KVF>()) store_logits(logit_row + t0 + 4 * g, x, row_ok ? t_end - t0 - 4 * g : 0);
+    if constexpr (kv_weights<KVF>()) logits.store(t0 + 4 * g, x, t_end, full);
     float bm = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
     bm = fmaxf(bm, shfl_xor_f(bm, 16));
     bm = fmaxf(bm, shfl_xor_f(bm, 32));

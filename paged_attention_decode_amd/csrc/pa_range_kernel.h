@@ -30,6 +30,8 @@
 #ifndef PA_RANGE_KERNEL_H_
 #define PA_RANGE_KERNEL_H_
 
+#include <type_traits>
+
 #include "pa_mx4.h"
 #include "pa_range.h"
 
@@ -212,8 +214,7 @@ __device__ __forceinline__ void range_wave_loop(const Phase1Args& a, int phys_fi
   // the result; the four rows are alike).  Where the caller gets the weights,
   // which are unrounded, a lane's own sum takes its place.
   f4_t o_l = (f4_t)0.f;
-  float* logit_row = nullptr;
-  if constexpr (kv_weights<KVF>()) logit_row = logits_of(a, b, kvh, row_ok ? r16 : 0);
+  const std::conditional_t<kv_weights<KVF>(), Logits, NoLogits> logits(a, b, kvh, r16);
   const _Float16 one16 = round16<KVF>(1.0f);
 
   const char* k_head = reinterpret_cast<const char*>(a.k) + (int64_t)kvh * a.skh * ES;
@@ -384,10 +385,8 @@ __device__ __forceinline__ void range_wave_loop(const Phase1Args& a, int phys_fi
     }
     if constexpr (kv_weights<KVF>()) {
 #pragma unroll
-      for (int s = 0; s < N; ++s) {
-        const int tk = t_begin + (jb + s * nw) * kBlockTokens + 4 * g;
-        store_logits(logit_row + tk, x[s], row_ok ? t_end - tk : 0);
-      }
+      for (int s = 0; s < N; ++s)
+        logits.store(t_begin + (jb + s * nw) * kBlockTokens + 4 * g, x[s], t_end, !MASKED);
     }
     float bm = kNegInf;
 #pragma unroll
