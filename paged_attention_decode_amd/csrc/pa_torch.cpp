@@ -727,7 +727,7 @@ void check_index(const torch::Tensor& block_table, const torch::Tensor& seq_lens
 torch::Tensor aligned_rows(const torch::Tensor& x) {
   const bool ok = x.stride(2) == 1 && x.stride(1) % 8 == 0 && x.stride(0) % 8 == 0 &&
                   reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
-  return ok ? x : x.contiguous().data_ptr() == x.data_ptr() ? x.clone(at::MemoryFormat::Contiguous) : x.contiguous();
+  return ok ? x : x.clone(at::MemoryFormat::Contiguous);
 }
 
 pad_kv_rows rows_desc(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& slots) {

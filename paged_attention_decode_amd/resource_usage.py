@@ -1,7 +1,6 @@
 """Register and scratch use of every decode-kernel instantiation, from the compiler.
 
-Compiles ``csrc/pa_decode.hip`` and ``csrc/pa_range.hip`` for gfx950 (device
-code only, the product flags of ``build.py``) with ``-Rpass-analysis=kernel-resource-usage`` and
+Compiles the sources of ``libpa_decode.so`` for gfx950 (device code only, the product flags of ``build.py``) with ``-Rpass-analysis=kernel-resource-usage`` and
 parses the remarks: per kernel VGPRs, AGPRs, SGPRs, scratch bytes per lane,
 SGPR and VGPR spill counts, occupancy (waves per SIMD) and static LDS.
 
@@ -37,14 +36,16 @@ FIELDS = {
 def _demangle_args(name: str) -> str:
     # _ZN3pad17pad_phase1_kernelILi128ELi1ELi0ELi0ELi0EEEvNS_10Phase1ArgsE -> <128, 1, 0, 0> (fp16 caches);
     # a fifth argument of 1-5 is printed as e4m3fn / e5m2 (fp8 caches, fp16 q),
-    # bf16, e4m3fn/bf16 / e5m2/bf16 (fp8 caches, bfloat16 q).
+    # bf16, e4m3fn/bf16 / e5m2/bf16 (fp8 caches, bfloat16 q), 6 and 7 as mx4 and
+    # mx4/bf16; 16 more marks a kernel that also writes its scores.
     args = re.findall(r"Li(\d+)E", name)
     # pad_range_kernel: <head_dim, block mode> and the format
     if len(args) in (3, 5):
         kvf = args.pop()
         if kvf != "0":
-            args.append({"1": "e4m3fn", "2": "e5m2", "3": "bf16", "4": "e4m3fn/bf16",
-                         "5": "e5m2/bf16"}.get(kvf, kvf))
+            name = {"1": "e4m3fn", "2": "e5m2", "3": "bf16", "4": "e4m3fn/bf16", "5": "e5m2/bf16", "6": "mx4",
+                    "7": "mx4/bf16"}.get(str(int(kvf) & 15), "fp16")
+            args.append(name + ("+weights" if int(kvf) & 16 else ""))
     return "<" + ", ".join(args) + ">" if args else name
 
 
