@@ -874,7 +874,7 @@ static int launch_impl(const void* q, const void* k, const void* v, const int32_
 }
 
 #ifndef PAD_TIMELINE
-// Floats of one row of scores: a table row's tokens, in whole vectors of four.
+// Floats of a query head's scores: a table row's tokens, in whole vectors of four.
 static int64_t logit_row_floats(const pad_decode_dims* d) { return ((int64_t)d->max_pages * d->page_size + 3) & ~3ll; }
 
 static size_t logits_bytes_of(const pad_decode_dims* d) {

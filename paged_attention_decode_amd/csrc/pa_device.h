@@ -93,8 +93,8 @@ struct Phase1Args {
   const uint8_t* vs;
   int64_t sksp, skss, sksh;
   int64_t svsp, svss, svsh;
-  // kKvWeights: every score in base-2 units, [batch * query heads] rows of
-  // slog floats by token, and log2 of each row's normaliser, [batch * query heads].
+  // kKvWeights: every score in base-2 units, slog floats per query head ([batch,
+  // kv heads, slog, group]), and log2 of each query head's normaliser [batch, hq].
   float* logits;
   float* lse;
   int64_t slog;
@@ -503,28 +503,29 @@ __device__ __forceinline__ void fp8x4_to_16x4(uint32_t w, uint32_t& lo, uint32_t
 template <int D>
 constexpr bool q_in_lds() { return D >= 256; }
 
-// Scores of kKvWeights calls: those of kv head kvh's rows, slog floats each, as a
-// buffer (below 2^32 bytes, which the launcher sees to).  Stores past its end are dropped,
-// so rows that do not exist need no branch: one around the stores kept the
-// compiler from waiting for the loads before them alone.
+// Scores of kKvWeights calls: kv head kvh's of a sequence, by token and row
+// within the token, as a buffer (below 2^32 bytes, which the launcher sees to).
+// Stores past its end are dropped, so rows that do not exist need no branch.  A
+// block's scores are consecutive (with a token's rows apart, the accumulation that
+// reads them took 10.9 us for 8.5 at 48 x [1, 6000] of 32/8 heads).  What the
+// stores cost the decode is the memory's: 18 MB of them beside 300 MB of K and V
+// 12 us, in any layout and with any cache policy tried.
 struct Logits {
   __amdgpu_buffer_rsrc_t r;
-  uint32_t row;  // the lane's row, or past the end
+  uint32_t row, step;  // the lane's row, or past the end; bytes of a token's scores
   __device__ __forceinline__ Logits(const Phase1Args& a, int b, int kvh, int r16) {
-    const uint32_t bytes = (uint32_t)(a.gqa * a.slog * 4);
-    r = make_rsrc(a.logits + ((int64_t)b * a.hq + kvh * a.gqa) * a.slog, bytes);
-    row = r16 < a.gqa ? (uint32_t)r16 * (uint32_t)a.slog * 4u : 0xffffffffu;
+    step = (uint32_t)a.gqa * 4u;
+    r = make_rsrc(a.logits + ((int64_t)b * a.hq + kvh * a.gqa) * a.slog, (uint32_t)(a.gqa * a.slog * 4));
+    row = r16 < a.gqa ? (uint32_t)r16 * 4u : 0xffffffffu;
   }
-  // Four consecutive scores from token t on, of which those below t_end are
-  // written; whole: all of the wave's are.
+  // Four consecutive tokens' scores from token t on, of which those below t_end
+  // are written; whole: all of the wave's are.
   __device__ __forceinline__ void store(int t, const float (&x)[4], int t_end, bool whole) const {
-    const uint32_t off = row == 0xffffffffu ? 0xfffffff0u : row + (uint32_t)t * 4u;
-    if (whole) {
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i4_t, f4_t{x[0], x[1], x[2], x[3]}), r, off, 0, 0);
-    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[i]), r, t + i < t_end ? off + 4u * i : 0xfffffff0u, 0, 0);
+    for (int i = 0; i < 4; ++i) {
+      const bool in = row != 0xffffffffu && (whole || t + i < t_end);
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[i]), r, in ? (uint32_t)(t + i) * step + row : 0xfffffff0u, 0,
+                                            0);
     }
   }
 };
