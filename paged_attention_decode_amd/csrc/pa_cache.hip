@@ -358,10 +358,13 @@ hipError_t launch_accumulate(const Phase1Args& p, float* weights, const int64_t*
 // targets below it, so no move can overwrite what another reads, and moves run
 // in any order.
 //
-// A workgroup selects for one unit; few barriers bound it, so every wave scans
-// the 256 counts of a digit by itself (one barrier a digit), and keys stay in
-// registers: they are read once, a round trip for the page ids and one for
-// weights and positions.
+// A workgroup selects for one unit; round trips and barriers bound it, so every
+// wave scans the 256 counts of a digit by itself (one barrier a digit), and keys
+// stay in registers: they are read once, a round trip for the page ids and one
+// for weights and positions.  64 x 2049 slots of 2 heads, one token to go: 11.3 us
+// with the move (20.8 + 4.8 with keys read again in each of three passes; 512
+// threads 12.6 for 12.2 of 1024).  16 x 5120 of 8 heads, 1024 to go: 16.9 us, and
+// the moves 28.8 us (33.3 one at a time), 4.7 TB/s, what a copy reaches.
 // ---------------------------------------------------------------------------
 struct EvictArgs {
   pad_kv_cache c;
@@ -420,22 +423,36 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int b, int h, cons
   const int64_t* st = is_v ? a.c.v_stride : a.c.k_stride;
   const int64_t* ss = is_v ? a.c.vs_stride : a.c.ks_stride;
   char* base = static_cast<char*>(is_v ? a.c.v : a.c.k) + (int64_t)h * st[2] * a.elem_bytes + c * sizeof(U);
-  for (int i = block * per + mine; i < m; i += blocks * per) {
-    const int2 mv = list[i];
-    const Place s = evict_place(a, b, mv.x), d = evict_place(a, b, mv.y);
-    *reinterpret_cast<U*>(base + (d.page * st[0] + d.at * st[1]) * a.elem_bytes) =
-        *reinterpret_cast<const U*>(base + (s.page * st[0] + s.at * st[1]) * a.elem_bytes);
-    if (c < a.scale_bytes) {
-      uint8_t* sb = (is_v ? a.c.v_scales : a.c.k_scales) + (int64_t)h * ss[2] + c;
-      sb[d.page * ss[0] + d.at * ss[1]] = sb[s.page * ss[0] + s.at * ss[1]];
+  // Four moves at a time: a round trip for the list, the page ids and the rows each.
+  constexpr int N = 4;
+  const int step = blocks * per;
+  for (int i0 = block * per + mine; i0 < m; i0 += N * step) {
+    int2 mv[N];
+    Place s[N], d[N];
+    U row[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) mv[j] = list[min(i0 + j * step, m - 1)];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      s[j] = evict_place(a, b, mv[j].x);
+      d[j] = evict_place(a, b, mv[j].y);
     }
-    if (c == 0) {
-      if (is_v) {
-        int32_t* p = a.c.positions + (int64_t)h * a.c.p_stride[2];
-        p[d.page * a.c.p_stride[0] + d.at * a.c.p_stride[1]] = p[s.page * a.c.p_stride[0] + s.at * a.c.p_stride[1]];
-      } else {
-        float* w = a.c.weights + (int64_t)h * a.c.w_stride[2];
-        w[d.page * a.c.w_stride[0] + d.at * a.c.w_stride[1]] = w[s.page * a.c.w_stride[0] + s.at * a.c.w_stride[1]];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      row[j] = *reinterpret_cast<const U*>(base + (s[j].page * st[0] + s[j].at * st[1]) * a.elem_bytes);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (i0 + j * step >= m) break;
+      *reinterpret_cast<U*>(base + (d[j].page * st[0] + d[j].at * st[1]) * a.elem_bytes) = row[j];
+      if (c < a.scale_bytes) {
+        uint8_t* sb = (is_v ? a.c.v_scales : a.c.k_scales) + (int64_t)h * ss[2] + c;
+        sb[d[j].page * ss[0] + d[j].at * ss[1]] = sb[s[j].page * ss[0] + s[j].at * ss[1]];
+      }
+      if (c == 0) {
+        const int64_t* ws = is_v ? a.c.p_stride : a.c.w_stride;  // 32-bit words either way
+        uint32_t* w = (is_v ? reinterpret_cast<uint32_t*>(a.c.positions) : reinterpret_cast<uint32_t*>(a.c.weights)) +
+                      (int64_t)h * ws[2];
+        w[d[j].page * ws[0] + d[j].at * ws[1]] = w[s[j].page * ws[0] + s[j].at * ws[1]];
       }
     }
   }
@@ -471,7 +488,7 @@ __global__ __launch_bounds__(THREADS) void pad_evict_select_kernel(const EvictAr
     return;
   }
   __shared__ int hist[4][256];
-  __shared__ int sm[2][WAVES];
+  __shared__ int2 sm[2][WAVES];
   __shared__ int2 own[kOwnMoves];
   for (int i = tid; i < 4 * 256; i += THREADS) hist[0][i] = 0;
 
@@ -518,10 +535,10 @@ __global__ __launch_bounds__(THREADS) void pad_evict_select_kernel(const EvictAr
       }
     }
     newest = wave_max_i32(newest);
-    if (lane == 0) sm[0][wave] = newest;
+    if (lane == 0) sm[0][wave].x = newest;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) newest = max(newest, sm[0][w]);
+    for (int w = 0; w < WAVES; ++w) newest = max(newest, sm[0][w].x);
     border = (int64_t)newest - a.e.recent;
     if constexpr (NR > 0) {
 #pragma unroll
@@ -558,6 +575,7 @@ __global__ __launch_bounds__(THREADS) void pad_evict_select_kernel(const EvictAr
   // The n-th largest key.
   uint32_t prefix = 0;
   int left = n;  // of the keys with this prefix, how many from the top
+  int equal = 0;  // keys with this prefix
 #pragma unroll
   for (int pass = 0; pass < 4; ++pass) {
     const int shift = 24 - 8 * pass;
@@ -571,40 +589,34 @@ __global__ __launch_bounds__(THREADS) void pad_evict_select_kernel(const EvictAr
     const int sum = c[0] + c[1] + c[2] + c[3];
     int above = wave_incl_scan_i32(sum, lane) - sum;
     int bin = -1;
-    int above_bin = 0;
+    int above_bin = 0, in_bin = 0;
 #pragma unroll
     for (int j = 3; j >= 0; --j) {
       if (above < left && left <= above + c[j]) {
         bin = 252 - 4 * lane + j;
         above_bin = above;
+        in_bin = c[j];
       }
       above += c[j];
     }
     const int who = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(bin >= 0));  // the keys counted are at least `left`
     prefix |= (uint32_t)__builtin_amdgcn_readlane(bin, who) << shift;
     left -= __builtin_amdgcn_readlane(above_bin, who);
+    equal = __builtin_amdgcn_readlane(in_bin, who);
   }
 
-  // `left` of the keys equal to it are kept, the lowest slots first.
+  // `left` of the keys equal to it are kept, the lowest slots first: where not
+  // all are, their order over the waves counts.
   const uint64_t below = (1ull << lane) - 1;
-  auto counts_before = [&](int count, int* place, int& total) {  // exclusive prefix over the waves
-    if (lane == 0) place[wave] = count;
+  int tie0 = 0;
+  if (equal != left) {
+    int ties = 0;
+    each([&](int, uint32_t k) { ties += (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(k == prefix)); });
+    if (lane == 0) sm[1][wave] = make_int2(ties, 0);
     __syncthreads();
-    int base = 0;
-    total = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const int c = place[w];
-      base += w < wave ? c : 0;
-      total += c;
-    }
-    return base;
-  };
-  int ties = 0, total;
-  each([&](int, uint32_t k) { ties += (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(k == prefix)); });
-  // (Two places in turn: a wave that writes one has passed a barrier that all
-  // reached after reading it.)
-  const int tie0 = counts_before(ties, sm[1], total);
+    for (int w = 0; w < WAVES; ++w) tie0 += w < wave ? sm[1][w].x : 0;
+  }
   int tie = tie0, movers = 0, holes = 0;
   auto classify = [&](int i, uint32_t k, uint64_t& moves, uint64_t& opens) {
     const int slot = first + i * 64;
@@ -620,9 +632,17 @@ __global__ __launch_bounds__(THREADS) void pad_evict_select_kernel(const EvictAr
     movers += (int)__builtin_popcountll(mv);
     holes += (int)__builtin_popcountll(op);
   });
-  int num_moves;
-  int mover = counts_before(movers, sm[0], num_moves);
-  int hole = counts_before(holes, sm[1], total);
+  // (Places in turn: every wave has passed a barrier since it read this one.)
+  if (lane == 0) sm[0][wave] = make_int2(movers, holes);
+  __syncthreads();
+  int mover = 0, hole = 0, num_moves = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const int2 x = sm[0][w];
+    mover += w < wave ? x.x : 0;
+    hole += w < wave ? x.y : 0;
+    num_moves += x.x;
+  }
   num_moves = (int)min((int64_t)num_moves, a.most);
   const bool mine = num_moves <= kOwnMoves;
   int2* list = mine ? own : a.moves + unit * a.most;

@@ -502,6 +502,72 @@ def test_another_stream_and_two_at_once():
     assert all(torch.equal(bits(a), bits(one)) for a in acc)
 
 
+def test_views_of_larger_buffers():
+    """Codes and scales of K and V in one buffer per page, tables and lengths as strided views: the same bits."""
+    case, (q, k, v, table, lens, s) = _state(MX4)
+    pages, ps, hkv, d = case.pages, 16, 2, 128
+    weights, positions = pad.kv_weights(pages, ps, hkv)
+    positions.copy_(torch.randperm(pages * ps, device="cuda").view(pages, ps, 1).expand(-1, -1, hkv))
+    code, scale = ps * hkv * d // 2, ps * hkv * d // 32
+    buf = torch.full((pages, 2 * (code + scale) + 64), 0x5a, dtype=torch.uint8, device="cuda")
+    step = buf.shape[1]
+
+    def view(at, width):
+        return buf.as_strided((pages, ps, hkv, width), (step, hkv * width, width, 1), at)
+
+    k2, v2, ks2, vs2 = view(0, d // 2), view(code, d // 2), view(2 * code, d // 32), view(2 * code + scale, d // 32)
+    for x, y in ((k2, k), (v2, v), (ks2, s["k_scale"]), (vs2, s["v_scale"])):
+        x.copy_(y)
+    state = torch.zeros(pages, hkv, 3, ps, 2, device="cuda")
+    w2 = state[:, :, 1, :, 0].transpose(1, 2)
+    p2 = torch.zeros(ps, pages, hkv, dtype=torch.int32, device="cuda").transpose(0, 1)
+    p2.copy_(positions)
+    wide = torch.full((len(case.lens), 2 * table.shape[1]), -1, dtype=torch.int32, device="cuda")
+    wide[:, ::2] = table
+    t2, l2 = wide[:, ::2], torch.stack([lens, lens + 7], 1)[:, 0]
+    rows = torch.randn(3, 2, hkv, d, dtype=torch.float16, device="cuda")
+    slots = torch.tensor([3, -1, 40], device="cuda")
+    tp = torch.tensor([900, 901, 902], dtype=torch.int32, device="cuda")
+    for kk, vv, a, b, w, p in ((k, v, s["k_scale"], s["v_scale"], weights, positions), (k2, v2, ks2, vs2, w2, p2)):
+        pad.paged_kv_append(rows[:, 0], rows[:, 1], kk, vv, slots, a, b, weights=w, positions=p, token_positions=tp)
+    assert torch.equal(bits(pad.paged_kv_read(k, v, slots, s["k_scale"], s["v_scale"])[1]),
+                       bits(pad.paged_kv_read(k2, v2, slots, ks2, vs2)[1]))
+    one = pad.paged_attention_decode_weights(q, k, v, weights, table, lens, **s)
+    two = pad.paged_attention_decode_weights(q, k2, v2, w2, t2, l2, k_scale=ks2, v_scale=vs2)
+    assert torch.equal(bits(one), bits(two)) and torch.equal(bits(weights), bits(w2))
+    assert torch.equal(bits(pad.paged_attention_decode_mx4(q, k, v, s["k_scale"], s["v_scale"], table, lens)),
+                       bits(pad.paged_attention_decode_mx4(q, k2, v2, ks2, vs2, t2, l2)))
+    n1 = pad.paged_kv_evict(k, v, weights, positions, table, lens, 30, 4, **s)
+    n2 = pad.paged_kv_evict(k2, v2, w2, p2, t2, l2, 30, 4, k_scale=ks2, v_scale=vs2)
+    assert torch.equal(n1, n2)
+    for x, y in ((k, k2), (v, v2), (s["k_scale"], ks2), (s["v_scale"], vs2), (weights, w2), (positions, p2)):
+        assert torch.equal(bits(x), bits(y))
+    assert (buf[:, -64:] == 0x5a).all() and (state[:, :, 0] == 0).all() and (state[..., 1] == 0).all()
+
+
+def test_sixteen_bit_caches_with_kv_interleaved():
+    """K and V as halves of one buffer, kv heads outermost: append, weights and eviction as on plain caches."""
+    ps, hkv, d, lens_l = 12, 3, 96, [50, 0, 7, 121]
+    table, pages, w, p = eviction_case(lens_l, hkv, ps, seed=8)
+    both = torch.randn(hkv, pages, ps, 2, d, dtype=torch.float16, device="cuda")
+    k2, v2 = both[:, :, :, 0].permute(1, 2, 0, 3), both[:, :, :, 1].permute(1, 2, 0, 3)
+    k1, v1 = k2.contiguous(), v2.contiguous()
+    lens = torch.tensor(lens_l, dtype=torch.int32, device="cuda")
+    dt = table.cuda()
+    q = torch.randn(4, 6, d, dtype=torch.float16, device="cuda")
+    w1, p1, w2, p2 = w.cuda(), p.cuda(), head_major(w.unsqueeze(-1)).squeeze(-1).cuda(), p.cuda()
+    rows = torch.randn(5, hkv, d, dtype=torch.float16, device="cuda")
+    slots = torch.tensor([0, 5, 12, 31, -2], dtype=torch.int32, device="cuda")
+    results = []
+    for k, v, ww, pp in ((k1, v1, w1, p1), (k2, v2, w2, p2)):
+        pad.paged_kv_append(rows, 2 * rows, k, v, slots)
+        out = pad.paged_attention_decode_weights(q, k, v, ww, dt, lens)
+        n = pad.paged_kv_evict(k, v, ww, pp, dt, lens, 20, 5)
+        results.append([out, n, k, v, ww, pp, *pad.paged_kv_read(k, v, slots)])
+    for x, y in zip(*results):
+        assert torch.equal(bits(x), bits(y))
+
+
 def test_empty_batch_and_empty_tables():
     k, v = (torch.zeros(2, 16, 2, 128, dtype=torch.float16, device="cuda") for _ in range(2))
     w, p = pad.kv_weights(2, 16, 2)
