@@ -18,8 +18,8 @@
  * (weights, eviction); two sequences that share one lose updates.
  *
  * Everything is asynchronous on `stream`, allocates nothing and can be captured.
- * Page ids outside [0, num_pages) read page 0 (decode, eviction); slots outside
- * the cache are skipped (append) or read as zeros (read).
+ * Page ids outside [0, num_pages) read page 0 and are not written to; slots
+ * outside the cache are skipped (append) or read as zeros (read).
  * Return codes are pa_decode.h's pad_status.  The operators have no
  * counterparts in the reference, whose callers fill fp16 caches themselves
  * (tests/kernel_test_utils.py).

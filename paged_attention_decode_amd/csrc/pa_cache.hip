@@ -316,7 +316,7 @@ __global__ __launch_bounds__(256) void pad_accumulate_kernel(const AccumulateArg
     float sum = 0.f;
 #pragma unroll 4
     for (int r = 0; r < a.gqa; ++r) sum += exp2_fast(x[r] - lse[r]);
-    *w = old + sum;
+    if (id >= 0 && id < a.num_pages) *w = old + sum;  // (not to page 0 for an id that is none)
     t += gridDim.x * 256;
     if (t < L) id = a.bt[b * a.sbb + (int64_t)page_at(t) * a.sbp];
   }
@@ -398,11 +398,14 @@ __device__ __forceinline__ int evict_page(const EvictArgs& a, int slot) {
 // Where a slot of sequence b lies.
 struct Place {
   int64_t page, at;
+  bool real;  // the table's id is a page (else page 0 is read, and nothing written)
 };
 __device__ __forceinline__ Place evict_place(const EvictArgs& a, int b, int slot) {
   const int page = evict_page(a, slot);
   Place p;
-  p.page = clamp_page(a.e.block_table[(int64_t)b * a.e.bt_stride[0] + (int64_t)page * a.e.bt_stride[1]], a.c.num_pages);
+  const int id = a.e.block_table[(int64_t)b * a.e.bt_stride[0] + (int64_t)page * a.e.bt_stride[1]];
+  p.page = clamp_page(id, a.c.num_pages);
+  p.real = p.page == id;
   p.at = slot - (int64_t)page * a.c.page_size;
   return p;
 }
@@ -443,6 +446,7 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int b, int h, cons
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       if (i0 + j * step >= m) break;
+      if (!s[j].real || !d[j].real) continue;
       *reinterpret_cast<U*>(base + (d[j].page * st[0] + d[j].at * st[1]) * a.elem_bytes) = row[j];
       if (c < a.scale_bytes) {
         uint8_t* sb = (is_v ? a.c.v_scales : a.c.k_scales) + (int64_t)h * ss[2] + c;

@@ -1,4 +1,5 @@
-// pa_decode.hip - gfx950 (MI355X) paged-attention decode: kernels + C ABI.
+// pa_decode.hip - gfx950 (MI355X) paged-attention decode: the per-unit kernel (its
+// code is in pa_phase1.h) over 16-bit and fp8 caches, and the C ABI.
 //
 // Operator contract: the reference oracle paged_attention_decode_reference
 // (src/reference.py:8-54) evaluated on fp16 inputs, output in fp16.

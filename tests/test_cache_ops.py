@@ -568,6 +568,27 @@ def test_sixteen_bit_caches_with_kv_interleaved():
         assert torch.equal(bits(x), bits(y))
 
 
+def test_wild_page_ids_write_nothing():
+    """An id outside the cache neither faults nor gives page 0 weights or rows."""
+    case, (q, k, v, table, lens, s) = _state(MX4)
+    weights, positions = (x.contiguous() for x in pad.kv_weights(case.pages, 16, 2))
+    bad = table.clone()
+    bad[0, 3], bad[0, 12], bad[1, 0] = 2**30, -1, case.pages
+    pad.paged_attention_decode_weights(q, k, v, weights, bad, lens, **s)
+    real = torch.zeros(case.pages, 16, dtype=torch.bool, device="cuda")
+    for b, n in enumerate(case.lens):
+        t = torch.arange(n, device="cuda")
+        ids = bad[b].long()[t // 16]
+        ok = (ids >= 0) & (ids < case.pages)
+        real[ids[ok], (t % 16)[ok]] = True
+    assert (weights[~real] == 0).all() and (weights[real] > 0).all()
+    before = [x.clone() for x in (k, v, *s.values(), weights, positions)]
+    n = pad.paged_kv_evict(k, v, weights, positions, bad, lens, 20, 0, **s)
+    assert n.tolist() == [20, 20, 1]
+    for x, y in zip((k, v, *s.values(), weights, positions), before):
+        assert torch.equal(bits(x)[~real.cpu()], bits(y)[~real.cpu()])
+
+
 def test_empty_batch_and_empty_tables():
     k, v = (torch.zeros(2, 16, 2, 128, dtype=torch.float16, device="cuda") for _ in range(2))
     w, p = pad.kv_weights(2, 16, 2)
