@@ -310,12 +310,12 @@ __global__ __launch_bounds__(256) void pad_accumulate_kernel(const AccumulateArg
   int id = a.bt[b * a.sbb + (int64_t)page_at(min(t, cap - 1)) * a.sbp];
   const uint32_t L = min((uint32_t)max(a.sl[(int64_t)b * a.ssl], 0), cap);
   while (t < L) {
-    const float* x = a.logits + row0 * a.slog + (int64_t)t * a.gqa;
+    const float* x = a.logits + row0 * a.slog + (int64_t)(t >> 2) * a.gqa * 4 + (t & 3);
     float* w = wh + clamp_page(id, a.num_pages) * a.swp + (int64_t)(t - page_at(t) * (uint32_t)a.ps) * a.sws;
     const float old = *w;
     float sum = 0.f;
 #pragma unroll 4
-    for (int r = 0; r < a.gqa; ++r) sum += exp2_fast(x[r] - lse[r]);
+    for (int r = 0; r < a.gqa; ++r) sum += exp2_fast(x[4 * r] - lse[r]);
     if (id >= 0 && id < a.num_pages) *w = old + sum;  // (not to page 0 for an id that is none)
     t += gridDim.x * 256;
     if (t < L) id = a.bt[b * a.sbb + (int64_t)page_at(t) * a.sbp];

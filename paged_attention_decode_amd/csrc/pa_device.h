@@ -94,7 +94,7 @@ struct Phase1Args {
   int64_t sksp, skss, sksh;
   int64_t svsp, svss, svsh;
   // kKvWeights: every score in base-2 units, slog floats per query head ([batch,
-  // kv heads, slog, group]), and log2 of each query head's normaliser [batch, hq].
+  // kv heads, slog / 4, group, 4]), and log2 of each query head's normaliser [batch, hq].
   float* logits;
   float* lse;
   int64_t slog;
@@ -503,32 +503,45 @@ __device__ __forceinline__ void fp8x4_to_16x4(uint32_t w, uint32_t& lo, uint32_t
 template <int D>
 constexpr bool q_in_lds() { return D >= 256; }
 
-// Scores of kKvWeights calls: kv head kvh's of a sequence, by token and row
-// within the token, as a buffer (below 2^32 bytes, which the launcher sees to).
-// Stores past its end are dropped, so rows that do not exist need no branch.  A
-// block's scores are consecutive (with a token's rows apart, the accumulation that
-// reads them took 10.9 us for 8.5 at 48 x [1, 6000] of 32/8 heads).  What the
-// stores cost the decode is the memory's: 18 MB of them beside 300 MB of K and V
-// 12 us, in any layout and with any cache policy tried.
+// Scores of kKvWeights calls: kv head kvh's of a sequence, as [token / 4][row][token
+// % 4], in a buffer (below 2^32 bytes, which the launcher sees to).  A lane's four
+// tokens of a row are one store and a block's scores consecutive: us of decode +
+// accumulation, 48 x [1, 6000] of 32/8 heads, fp8: by row 65.7 + 10.9, by token 65.7 +
+// 8.5, so 63.4 + 8.8.  Stores past the buffer's end are dropped, so rows that do not
+// exist need no branch (with one, 64 x 4096 of 12/2 took 58.3 us for 54.2).  Of
+// what the stores add (18 MB beside 300 MB of K and V, 9 us) two thirds are the
+// memory's: stored over and over to the same 4 KB they add 3.
 struct Logits {
   __amdgpu_buffer_rsrc_t r;
-  uint32_t row, step;  // the lane's row, or past the end; bytes of a token's scores
+  uint32_t row, step;  // the lane's row, or past the end; bytes of four tokens' scores
   __device__ __forceinline__ Logits(const Phase1Args& a, int b, int kvh, int r16) {
-    step = (uint32_t)a.gqa * 4u;
+    step = (uint32_t)a.gqa * 16u;
     r = make_rsrc(a.logits + ((int64_t)b * a.hq + kvh * a.gqa) * a.slog, (uint32_t)(a.gqa * a.slog * 4));
-    row = r16 < a.gqa ? (uint32_t)r16 * 4u : 0xffffffffu;
+    row = r16 < a.gqa ? (uint32_t)r16 * 16u : 0xffffffffu;
   }
-  // Four consecutive tokens' scores from token t on, of which those below t_end
-  // are written; whole: all of the wave's are.
-  __device__ __forceinline__ void store(int t, const float (&x)[4], int t_end, bool whole) const {
+  // Four consecutive tokens' scores from token t on, those below t_end.  BY4: t is
+  // a multiple of four and t_end one too or the sequence's end, behind which
+  // scores are not read.
+  template <bool BY4>
+  __device__ __forceinline__ void store(int t, const float (&x)[4], int t_end) const {
+    const bool live = row != 0xffffffffu;
+    if constexpr (BY4) {
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i4_t, f4_t{x[0], x[1], x[2], x[3]}), r,
+                                             live && t < t_end ? (uint32_t)(t >> 2) * step + row : 0xfffffff0u, 0, 0);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool in = row != 0xffffffffu && (whole || t + i < t_end);
-      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[i]), r, in ? (uint32_t)(t + i) * step + row : 0xfffffff0u, 0,
-                                            0);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t s = (uint32_t)(t + i);
+        __builtin_amdgcn_raw_buffer_store_b32(
+            __float_as_uint(x[i]), r, live && t + i < t_end ? (s >> 2) * step + row + (s & 3) * 4u : 0xfffffff0u, 0, 0);
+      }
     }
   }
 };
+
+// Block modes whose items begin and end at multiples of four tokens (pages do).
+template <int MODE>
+constexpr bool logits_by4() { return MODE == kModeUniform || MODE >= kModeSubpage + 2; }
 
 struct NoLogits {
   __device__ __forceinline__ NoLogits(const Phase1Args&, int, int, int) {}

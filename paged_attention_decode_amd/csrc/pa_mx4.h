@@ -281,7 +281,7 @@ __device__ __forceinline__ void wave_loop_mx4(const Phase1Args& a, const int32_t
     }
     if constexpr (kv_weights<KVF>()) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) logits.store(t0 + 16 * u + 4 * g, x[u], t_end, t0 + 32 <= t_end);
+      for (int u = 0; u < 2; ++u) logits.template store<logits_by4<MODE>()>(t0 + 16 * u + 4 * g, x[u], t_end);
     }
     float bm = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                      fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));

@@ -294,7 +294,7 @@ __device__ __forceinline__ void wave_loop_mfma(const Phase1Args& a, int phys_fir
         if (!valid) t.v[i].zero();  // stale cache slots may hold NaN/Inf
       }
     }
-    if constexpr (kv_weights<KVF>()) logits.store(t0 + 4 * g, x, t_end, full);
+    if constexpr (kv_weights<KVF>()) logits.template store<logits_by4<MODE>()>(t0 + 4 * g, x, t_end);
     float bm = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
     bm = fmaxf(bm, shfl_xor_f(bm, 16));
     bm = fmaxf(bm, shfl_xor_f(bm, 32));

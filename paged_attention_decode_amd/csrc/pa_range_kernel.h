@@ -386,7 +386,7 @@ __device__ __forceinline__ void range_wave_loop(const Phase1Args& a, int phys_fi
     if constexpr (kv_weights<KVF>()) {
 #pragma unroll
       for (int s = 0; s < N; ++s)
-        logits.store(t_begin + (jb + s * nw) * kBlockTokens + 4 * g, x[s], t_end, !MASKED);
+        logits.template store<logits_by4<MODE>()>(t_begin + (jb + s * nw) * kBlockTokens + 4 * g, x[s], t_end);
     }
     float bm = kNegInf;
 #pragma unroll
