@@ -48,7 +48,8 @@ extern "C" {
  *     slot and kv head.
  *   weights, w_stride: NULL, or where the softmax weights of every token, summed
  *     over the query heads of its kv head, are added (strides in elements).
- *   logits, logits_bytes: scratch of pad_cache_logits_bytes(), with weights.
+ *   logits, logits_bytes: scratch of pad_cache_logits_bytes(), with weights (a
+ *     table row's tokens times the group of query heads: below 2^30).
  * Scratch (workspace, counters): pad_cache_scratch(); with less than that a call
  * may run another kernel, or return PAD_ERR_WORKSPACE. */
 typedef struct pad_cache_call {

@@ -914,6 +914,9 @@ static int launch_cache_call(const pad_cache_call* cc, const pad_decode_dims* d,
   }
   // The launch counts the tokens of a table row in 32 bits.
   if ((int64_t)d->max_pages * d->page_size > INT32_MAX - 4096) return PAD_ERR_INVALID_SHAPE;
+  // A kv head's scores are one buffer with 32-bit offsets.
+  if (cc->weights && logit_row_floats(d) * (d->num_q_heads / d->num_kv_heads) >= (1ll << 30) - 1024)
+    return PAD_ERR_INVALID_SHAPE;
   Launch L;
   st = setup_launch(c.q, c.k_cache, c.v_cache, c.block_table, c.seq_lens, nullptr, nullptr, c.out, c.workspace,
                     c.workspace_bytes, c.counters, c.num_counters, d, c.scale, c.num_splits, 0, true, &L,
@@ -933,8 +936,6 @@ static int launch_cache_call(const pad_cache_call* cc, const pad_decode_dims* d,
   L.a.svss = cc->vs_stride[1];
   L.a.svsh = cc->vs_stride[2];
   if (cc->weights) {
-    // A kv head's scores are one buffer with 32-bit offsets.
-    if (logit_row_floats(d) * (d->num_q_heads / d->num_kv_heads) >= (1ll << 30) - 1024) return PAD_ERR_INVALID_SHAPE;
     if (!cc->logits || cc->logits_bytes < logits_bytes_of(d)) return PAD_ERR_WORKSPACE;
     L.a.slog = logit_row_floats(d);
     L.a.logits = reinterpret_cast<float*>(((uintptr_t)cc->logits + 255u) & ~(uintptr_t)255u);

@@ -1,4 +1,4 @@
-"""The C ABI of the cache operators (include/pa_cache.h): declarations, sizes and refusals, without a GPU."""
+"""The C ABI of the cache operators (include/pa_cache.h): declarations, sizes and refusals (no GPU), and a call."""
 
 from __future__ import annotations
 
@@ -6,6 +6,8 @@ import ctypes
 import math
 import os
 import re
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -152,6 +154,7 @@ def test_logits_bytes():
     ({"engine": 1}, {}, FORMAT), ({"kv_format": FP16}, {}, FORMAT), ({"kv_format": 77}, {}, FORMAT),
     ({"kv_format": FP16, "engine": 1, "weights": PTR}, {}, FORMAT), ({"k_scales": None}, {}, NULL),
     ({}, {"page_size": 1 << 20, "max_pages": 1 << 12}, SHAPE), ({}, {"hkv": 3}, GQA),
+    ({"weights": PTR}, {"page_size": 1 << 16, "max_pages": 1 << 12}, SHAPE),
 ])
 def test_decode_refusals(call, dims, status):
     dims = dict(dims)
@@ -175,6 +178,66 @@ def test_decode_refuses_rows_of_eight_bytes():
     c.k_scales = c.v_scales = PTR
     assert _native.capi().pad_cache_decode(c, dm, None) == ALIGN
     assert _native.capi().pad_cache_decode(None, dm, None) == NULL
+
+
+def test_structures_match_the_header(tmp_path):
+    gcc = shutil.which("gcc")
+    if gcc is None:
+        pytest.skip("gcc not found")
+    structs = {"pad_cache_call": _native.PadCacheCall, "pad_kv_cache": _native.PadKvCache,
+               "pad_kv_rows": _native.PadKvRows, "pad_kv_evict_call": _native.PadKvEvictCall}
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "pa_cache.h"', "int main(void) {"]
+    for cname, py in structs.items():
+        lines.append(f'  printf("{cname} sizeof %zu\\n", sizeof({cname}));')
+        for fname, _ in py._fields_:
+            lines.append(f'  printf("{cname} {fname} %zu\\n", offsetof({cname}, {fname}));')
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join([*lines, "  return 0;", "}"]) + "\n")
+    subprocess.run([gcc, "-std=c99", f"-I{os.path.dirname(HEADER)}", str(src), "-o", str(exe)], check=True)
+    for line in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines():
+        cname, field, value = line.split()
+        py = structs[cname]
+        want = ctypes.sizeof(py) if field == "sizeof" else getattr(py, field).offset
+        assert int(value) == want, (cname, field, int(value), want)
+
+
+@pytest.mark.gpu
+def test_decode_through_the_c_abi():
+    """Caller-owned scratch of the queried sizes: the package's bits, with weights, twice from the same counters."""
+    import paged_attention_decode_amd as pad
+    from tests.cache_helpers import Case
+
+    case = Case([900, 3, 0, 64], 8, 2, 128, 16, "fp16", "mx4", seed=5)
+    q, k, v, table, lens, s = case.gpu()
+    acc = torch.zeros(case.pages, 16, 2, device="cuda")
+    want = pad.paged_attention_decode_weights(q, k, v, acc, table, lens, **s)
+    lib, out, got = _native.capi(), torch.empty_like(want), torch.zeros_like(acc)
+    dm = _native.dims_for(q, k, v, table, lens, out)
+    ws, logits, count = ctypes.c_size_t(), ctypes.c_size_t(), ctypes.c_int64()
+    assert lib.pad_cache_scratch(dm, MX4, 0, 0, ctypes.byref(ws), ctypes.byref(count)) == 0
+    assert lib.pad_cache_scratch(dm, 99, 0, 0, ctypes.byref(ws), ctypes.byref(count)) == FORMAT
+    assert lib.pad_cache_logits_bytes(dm, ctypes.byref(logits)) == 0
+    scratch = torch.empty(max(ws.value, 1), dtype=torch.uint8, device="cuda")
+    counters = torch.zeros(max(count.value, 1), dtype=torch.int32, device="cuda")
+    scores = torch.empty(logits.value, dtype=torch.uint8, device="cuda")
+    c = _native.PadCacheCall()
+    for name, t in (("q", q), ("k_cache", k), ("v_cache", v), ("block_table", table), ("seq_lens", lens), ("out", out),
+                    ("workspace", scratch), ("counters", counters)):
+        setattr(c.call, name, t.data_ptr())
+    c.call.workspace_bytes, c.call.num_counters = scratch.numel(), counters.numel()
+    c.call.kv_format, c.call.scale = MX4, case.scale
+    c.k_scales, c.v_scales = s["k_scale"].data_ptr(), s["v_scale"].data_ptr()
+    c.ks_stride[:], c.vs_stride[:] = s["k_scale"].stride()[:3], s["v_scale"].stride()[:3]
+    c.weights, c.logits, c.logits_bytes = got.data_ptr(), scores.data_ptr(), scores.numel()
+    c.w_stride[:] = got.stride()
+    stream = torch.cuda.current_stream().cuda_stream
+    for times in (1, 2):
+        assert lib.pad_cache_decode(c, dm, stream) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and (counters == 0).all()
+    assert torch.equal(got, acc + acc)
+    c.logits_bytes -= 300
+    assert lib.pad_cache_decode(c, dm, stream) == WORKSPACE
 
 
 # ------------------------------------------------------------------ the oracle itself
